@@ -136,6 +136,68 @@ void nvllm_lightning(float* out, float* ss, const float* q, const float* k, cons
 void nvllm_expert_ff(float* out, int* choice, float* score, const float* in, const float* z, const float* gate, const float* up, const float* down,
                      int dim, int ff, int experts, int top, int elem_bytes, int num_tokens);
 
+/* Linear attention by the gated delta rule: per value head h, with query and key head h / (heads / qk_heads), token by token
+ *     S <- exp(g) S;   u = beta (v - S^T k);   S <- S + k u^T;   out = scale S^T q,
+ * q and k divided by sqrt(sum of their squares + norm_eps) first when norm_eps > 0.  state: fp32 [n_slots][heads][dim][vdim], a
+ * sequence's slot is its id in seq_ids, empty at position 0; slots that the batch does not name stay as they are.  q, k: rows of
+ * [qk_heads][dim], v: rows of [heads][vdim], the first of token t at element t * q_ld, t * k_ld, t * v_ld; out [num_tokens][heads][vdim];
+ * elem_bytes 4: fp32, 2: bf16 (out is rounded once).  g (logarithm of the decay, at most 0; -infinity empties the state) and beta: fp32
+ * [num_tokens][heads].  A sequence's tokens lie side by side at consecutive positions.  States and all sums in fp32.
+ * dim at most 256.  out and state overlap nothing else.  Enqueued on the library stream; workspaces are the library's own.  Host
+ * arrays may be reused on return.  Returns 0 or a refusal (below; nothing is enqueued then): NVLLM_BAD_ARGUMENT for null pointers,
+ * sizes that are not positive, strides shorter than a row, pointers that are not multiples of their elements; NVLLM_BAD_SIZE;
+ * NVLLM_BAD_INDEX for a sequence id outside the slots, a negative position, a sequence whose tokens are apart; NVLLM_CAPTURED. */
+int nvllm_gated_delta(void* out, const void* q, const void* k, const void* v, const float* g, const float* beta, float* state, const int* seq_ids, const int* pos_arr,
+                      int n_slots, float scale, float norm_eps, int qk_heads, int heads, int dim, int vdim, int q_ld, int k_ld, int v_ld, int elem_bytes, int num_tokens);
+
+/* ------------------------------------------------ what branching sequences remember */
+/* No counterpart in the reference, whose sequences never share or move anything.  A sequence that branches (several samples of
+ * one prompt, beams) takes its past along: the table of its blocks by nvllm_fork_tables, and its states, if it has some, by
+ * nvllm_copy_states or nvllm_copy_model_states.  Like every operator these enqueue on the library stream, so they come behind the
+ * passes that were enqueued before and in front of later ones; the host's records change at once.
+ *
+ * What these entry points and nvllm_gated_delta answer when they refuse.  A call that refuses changes nothing. */
+enum {
+    NVLLM_BAD_ARGUMENT = -1, /* null, negative, or twice the same record                               */
+    NVLLM_BAD_SIZE = -2,     /* sizes beyond the limits, or a pool that is not the library's           */
+    NVLLM_BAD_INDEX = -3,    /* an id out of range, two values for one slot, a block that is not in use */
+    NVLLM_NO_BLOCKS = -4,    /* the pool has too few free blocks                                       */
+    NVLLM_NO_MEMORY = -5,
+    NVLLM_CAPTURED = -6      /* nvllm_stream() is being captured: their host arrays would be read again at a replay */
+};
+
+/* Slot to[i] <- slot from[i] for all i < n, in each of n_layers arrays [n_slots][slot_bytes] that lie behind one another, as if all
+ * slots were read before any is written: from and to may overlap (beams that change places), no slot occurs twice in `to`. */
+int nvllm_copy_states(void* state, size_t slot_bytes, int n_layers, int n_slots, const int* from, const int* to, int n);
+/* The same for what a loaded model keeps per sequence id (nvllm_init_model_states; ids below the room made so far).  0 at once for
+ * models that keep nothing. */
+int nvllm_copy_model_states(const Weights* w, const int* from, const int* to, int n);
+/* The same for blocks of a pool, in every layer, keys and values.  Any pool of this library. */
+int nvllm_copy_blocks(KVCacheManager* mgr, const int* from, const int* to, int n);
+
+/* Tables for n branches of a sequence that has `positions` positions in `from`.  Whole blocks are shared: they have one user more
+ * for each branch, and free_block() gives a block back to the pool when its last user frees it.  If the last block is
+ * part filled, every branch gets a copy of its own (allocated in the branches' order).  Branches and the sequence itself may go on
+ * appending; nobody may write into positions in front of the branch.  to[i]->block_indices has room for the blocks of
+ * `positions`; num_blocks is set. */
+int nvllm_fork_tables(KVCacheManager* mgr, const BlockTable* from, int positions, BlockTable** to, int n);
+/* Tables that have the block (0: it is free), as far as nvllm_fork_tables made them; or a refusal. */
+int nvllm_block_users(const KVCacheManager* mgr, int block);
+/* free_block() on every block of a table, the last one first; the table is empty then. */
+int nvllm_free_table(KVCacheManager* mgr, BlockTable* table);
+
+/* Moves blocks in use to the lowest numbers, in the order of theirs, and writes the given tables anew; the free blocks are then
+ * taken lowest first, as in a new pool.  A block that is in use and in none of the tables, or that has more users than tables
+ * are given, stays where it is.  Returns the number of blocks moved, or a refusal.  No pass that was given the old
+ * tables may be enqueued later. */
+int nvllm_compact_blocks(KVCacheManager* mgr, BlockTable** tables, int n);
+
+/* A pool in memory of the caller's (16-byte aligned, HBM): [n_layers][num_blocks][block_size][n_kv_heads][head_dim] elements each for
+ * keys and values, fp32 rows (elem_bytes 4) or fp16 pages (2; block_size 16, head_dim a multiple of 16, whose values have to be
+ * finite from the start).  Used like one of init_kv_cache_manager(); free_kv_cache_manager() leaves the memory alone.  n_kv_heads: the
+ * heads that this process stores. */
+int nvllm_attach_kv_pool(KVCacheManager* mgr, int block_size, int num_blocks, int n_layers, int n_kv_heads, int head_dim, int elem_bytes, void* pool_k, void* pool_v);
+
 /* -------------------------------------------------- one launch per decode step */
 /* No counterpart in the reference, whose layer loop (src/model.c:358-394) calls one operator
  * after the other.  With the switch on (off by default; environment NVLLM_DECODE_CHAIN=1 turns it

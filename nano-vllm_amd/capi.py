@@ -182,6 +182,15 @@ _HIP_ONLY = {
                                     _I, _I, _I, _I, _I, _I, _I, _I]),
     "nvllm_lightning": (_V, [_P, _P, _P, _P, _P, _P, _P, C.POINTER(C.c_float), _P, c_int_p, c_int_p, _I, _I, _I, _I, _I]),
     "nvllm_expert_ff": (_V, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I]),
+    "nvllm_gated_delta": (_I, [_P, _P, _P, _P, _P, _P, _P, c_int_p, c_int_p, _I, _F, _F, _I, _I, _I, _I, _I, _I, _I, _I, _I]),
+    "nvllm_copy_states": (_I, [_P, C.c_size_t, _I, _I, c_int_p, c_int_p, _I]),
+    "nvllm_copy_model_states": (_I, [C.POINTER(Weights), c_int_p, c_int_p, _I]),
+    "nvllm_copy_blocks": (_I, [C.POINTER(KVCacheManager), c_int_p, c_int_p, _I]),
+    "nvllm_fork_tables": (_I, [C.POINTER(KVCacheManager), C.POINTER(BlockTable), _I, C.POINTER(C.POINTER(BlockTable)), _I]),
+    "nvllm_block_users": (_I, [C.POINTER(KVCacheManager), _I]),
+    "nvllm_free_table": (_I, [C.POINTER(KVCacheManager), C.POINTER(BlockTable)]),
+    "nvllm_compact_blocks": (_I, [C.POINTER(KVCacheManager), C.POINTER(C.POINTER(BlockTable)), _I]),
+    "nvllm_attach_kv_pool": (_I, [C.POINTER(KVCacheManager), _I, _I, _I, _I, _I, _I, _P, _P]),
     "nvllm_prof_enable": (_V, [_I]),
     "nvllm_prof_reset": (_V, []),
     "nvllm_prof_num_classes": (_I, []),

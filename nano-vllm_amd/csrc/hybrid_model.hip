@@ -73,6 +73,8 @@ public:
     }
     void init_kv(KVCacheManager* mgr, int block_size, int num_blocks) override;
     void init_states(int slots) override;
+    std::vector<SlotArrays> states() const override;
+    int state_slots() const override { return slots_; }
     void forward(const PassArgs& a) override;
 
 private:
@@ -425,8 +427,20 @@ KvPages HybridModel::pages(const KVCacheManager* mgr, int run) const {
 }
 void HybridModel::init_kv(KVCacheManager* mgr, int block_size, int num_blocks) {
     size_t bytes = 0;
-    for (size_t r = 0; r < source_.size(); r++) bytes += pool_bytes((int)r, block_size, num_blocks);
-    init_block_pool(mgr, block_size, num_blocks, bytes);
+    std::vector<SlotArrays> arrays;
+    for (size_t r = 0; r < source_.size(); r++) {
+        const MixerSizes& m = layers_[source_[r]].m;
+        if (!m.lightning) add_kv_pages(arrays, bytes, f32_ ? 4 : 2, block_size, num_blocks, m.groups, m.dim, m.vdim);
+        bytes += pool_bytes((int)r, block_size, num_blocks);
+    }
+    init_block_pool(mgr, block_size, num_blocks, bytes, arrays);
+}
+
+std::vector<SlotArrays> HybridModel::states() const {
+    std::vector<SlotArrays> all;
+    for (const auto& r : states_)
+        if (r.slot_bytes) all.push_back(SlotArrays{r.mem, r.slot_bytes, 0, 1});
+    return all;
 }
 
 void HybridModel::init_states(int slots) {

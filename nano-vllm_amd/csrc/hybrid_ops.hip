@@ -68,7 +68,9 @@ using namespace nvllm;
 extern "C" {
 
 void nvllm_window_pool_init(KVCacheManager* mgr, int block_size, int num_blocks, int kv_heads, int dim, int vdim, int elem_bytes) {
-    init_block_pool(mgr, block_size, num_blocks, kv_pages_bytes(elem_bytes, block_size, num_blocks, kv_heads, dim, vdim));
+    std::vector<SlotArrays> arrays;
+    add_kv_pages(arrays, 0, elem_bytes, block_size, num_blocks, kv_heads, dim, vdim);
+    init_block_pool(mgr, block_size, num_blocks, kv_pages_bytes(elem_bytes, block_size, num_blocks, kv_heads, dim, vdim), arrays);
 }
 
 void nvllm_conv_rope(float* q, const float* raw, const float* taps, int n_taps, void* state, KVCacheManager* mgr, BlockTable** block_tables, int* seq_ids,

@@ -353,7 +353,12 @@ LatentPool LatentHyperModel::pool(const KVCacheManager* mgr, int run) const {
 }
 
 void LatentHyperModel::init_kv(KVCacheManager* mgr, int block_size, int num_blocks) {
-    init_block_pool(mgr, block_size, num_blocks, pool_bytes(block_size, num_blocks, (int)runs_.size()));
+    std::vector<SlotArrays> arrays;
+    for (size_t r = 0; r < runs_.size(); r++) {
+        const Mixer& m = layers_[runs_[r]].m;
+        arrays.push_back(SlotArrays{(void*)pool_bytes(block_size, num_blocks, (int)r), latent_pool_bytes(latent_pool(nullptr, f32_ ? 4 : 2, block_size, m.rank, m.rot), 1), 0, 1});
+    }
+    init_block_pool(mgr, block_size, num_blocks, pool_bytes(block_size, num_blocks, (int)runs_.size()), arrays);
 }
 
 // The pass with its tokens in another order: portions of several tokens first, then the single ones, whose products with W_uk and W_uv

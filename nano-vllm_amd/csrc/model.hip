@@ -698,6 +698,18 @@ void nvllm_init_model_states(const Weights* w, int n_slots) {
     if (m && m->dir) m->dir->init_states(n_slots);
 }
 
+int nvllm_copy_model_states(const Weights* w, const int* from, const int* to, int n) {
+    if (!w || n < 0 || (n > 0 && (!from || !to))) return NVLLM_BAD_ARGUMENT;
+    const ModelPriv* m = (const ModelPriv*)w->_data_buffer;
+    if (n == 0 || !m || !m->dir) return 0;
+    try {
+        const std::vector<SlotArrays> states = m->dir->states();
+        return states.empty() ? 0 : copy_slots(states, m->dir->state_slots(), from, to, n);
+    } catch (const std::bad_alloc&) {
+        return NVLLM_NO_MEMORY;
+    }
+}
+
 void nvllm_free_model(Weights* w) {
     if (!w || !w->_data_buffer) return;
     ModelPriv* m = (ModelPriv*)w->_data_buffer;

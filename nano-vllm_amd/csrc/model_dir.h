@@ -11,6 +11,7 @@
 
 #include "json.h"
 #include "nvllm_internal.h"
+#include "sequence_memory.h"
 #include "step_arrays.h"
 
 namespace nvllm {
@@ -70,6 +71,9 @@ public:
     virtual void init_kv(KVCacheManager* mgr, int block_size, int num_blocks) = 0;
     // room for the state that `slots` sequences carry from token to token (a sequence's slot is its id)
     virtual void init_states(int slots) { (void)slots; }
+    // those states, layer run by layer run
+    virtual std::vector<SlotArrays> states() const { return {}; }
+    virtual int state_slots() const { return 0; }
     virtual void forward(const PassArgs& a) = 0;
 };
 
@@ -97,8 +101,9 @@ typedef DirModel* (*DirModelLoader)(const ModelDir& dir, Config* p);
 DirModel* load_latent_hyper_model(const ModelDir& dir, Config* p);   // latent_model.hip
 DirModel* load_hybrid_model(const ModelDir& dir, Config* p);         // hybrid_model.hip
 
-// ops_api.hip: host bookkeeping of a block pool whose storage is ONE HBM buffer of `bytes` bytes (pool_v stays null)
-void init_block_pool(KVCacheManager* mgr, int block_size, int num_blocks, size_t bytes);
+// ops_api.hip: host bookkeeping of a block pool whose storage is ONE HBM buffer of `bytes` bytes (pool_v stays null); arrays: where
+// its blocks lie, as offsets into the buffer
+void init_block_pool(KVCacheManager* mgr, int block_size, int num_blocks, size_t bytes, const std::vector<SlotArrays>& arrays);
 size_t block_pool_bytes(const KVCacheManager* mgr);   // of such a pool; 0 for any other
 // model.hip: the folder model loaded last, if its Config says these numbers
 DirModel* current_dir_model(int n_layers, int n_kv_heads, int head_dim);

@@ -142,6 +142,7 @@ enum WsSlot {
     WS_F32_A,       // fp32 models: activations between operators
     WS_F32_B,
     WS_F32_C,
+    WS_DELTA,       // gated delta rule: what a pass's chunks need of each other, before the states go through them
     WS_COUNT
 };
 void* ws_get(WsSlot slot, size_t bytes);
@@ -202,6 +203,9 @@ enum ProfClass {
     PC_GEMM_SHARED_UP,   // ... the shared expert's ...
     PC_GEMM_SHARED_DOWN,
     PC_MOE_COMBINE,      // ... and the sum of their results
+    PC_DELTA,            // gated delta rule: portions of several tokens ...
+    PC_DELTA_TOK,        // ... and single tokens
+    PC_SLOT_COPY,        // blocks and states copied in every layer
     PC_COUNT
 };
 hipEvent_t prof_start_event();   // events of the enclosing ProfScope, or null when timing is off

@@ -4,6 +4,7 @@
 #include <algorithm>
 #include <array>
 #include <cstring>
+#include <new>
 #include <unordered_map>
 #include <vector>
 
@@ -11,6 +12,7 @@
 #include "latent_attention.h"
 #include "model_dir.h"
 #include "nvllm_internal.h"
+#include "sequence_memory.h"
 #include "step_arrays.h"
 
 namespace nvllm {
@@ -20,20 +22,35 @@ namespace nvllm {
 struct PoolInfo {
     int elem_bytes;
     int n_layers, n_kv_heads, head_dim;
+    bool owned;   // by the library: free_kv_cache_manager frees the memory
 };
-// Block pools of models that lay them out themselves: bytes behind pool_k.
-static std::unordered_map<const void*, size_t>& block_pools() {
-    static std::unordered_map<const void*, size_t> m;
+// Block pools of models that lay them out themselves: bytes behind pool_k, and where the blocks lie.
+struct BlockPool {
+    size_t bytes;
+    std::vector<SlotArrays> arrays;
+};
+static std::unordered_map<const void*, BlockPool>& block_pools() {
+    static std::unordered_map<const void*, BlockPool> m;
     return m;
 }
 size_t block_pool_bytes(const KVCacheManager* mgr) {
     auto it = block_pools().find(mgr->pool_k);
-    return it == block_pools().end() ? 0 : it->second;
+    return it == block_pools().end() ? 0 : it->second.bytes;
 }
 
 static std::unordered_map<const void*, PoolInfo>& pools() {
     static std::unordered_map<const void*, PoolInfo> m;
     return m;
+}
+
+std::vector<SlotArrays> pool_arrays(const KVCacheManager* mgr) {
+    const auto own = block_pools().find(mgr->pool_k);
+    if (own != block_pools().end()) return own->second.arrays;
+    const auto it = pools().find(mgr->pool_k);
+    if (it == pools().end()) return {};
+    const PoolInfo& p = it->second;
+    const size_t block = (size_t)mgr->block_size * p.n_kv_heads * p.head_dim * p.elem_bytes;
+    return {SlotArrays{mgr->pool_k, block, block * mgr->num_blocks, p.n_layers}, SlotArrays{mgr->pool_v, block, block * mgr->num_blocks, p.n_layers}};
 }
 
 KvPoolView pool_view(const KVCacheManager* mgr, int n_kv_heads, int head_dim) {
@@ -378,11 +395,31 @@ void init_kv_cache_manager(KVCacheManager* mgr, int block_size, int num_blocks, 
     HIP_CHECK(hipMemsetAsync(pv, 0, elems * eb, rt().stream));
     mgr->pool_k = (float*)pk;
     mgr->pool_v = (float*)pv;
-    pools()[pk] = PoolInfo{eb, n_layers, n_kv_heads, head_dim};
+    pools()[pk] = PoolInfo{eb, n_layers, n_kv_heads, head_dim, true};
+}
+
+int nvllm_attach_kv_pool(KVCacheManager* mgr, int block_size, int num_blocks, int n_layers, int n_kv_heads, int head_dim, int elem_bytes, void* pool_k, void* pool_v) {
+    if (!mgr || !pool_k || !pool_v || pool_k == pool_v || block_size <= 0 || num_blocks <= 0 || n_layers <= 0 || n_kv_heads <= 0 || head_dim <= 0) return NVLLM_BAD_ARGUMENT;
+    if (elem_bytes != 2 && elem_bytes != 4) return NVLLM_BAD_SIZE;
+    if (elem_bytes == 2 && (block_size != KV16_PAGE_KEYS || head_dim % 16 != 0)) return NVLLM_BAD_SIZE;   // (pages)
+    if ((long)num_blocks * block_size > 0x7fffffff) return NVLLM_BAD_SIZE;   // (rows of a pool are ints)
+    if (((size_t)pool_k | (size_t)pool_v) % 16 || block_pools().count(pool_k)) return NVLLM_BAD_ARGUMENT;
+    const auto known = pools().find(pool_k);
+    if (known != pools().end() && known->second.owned) return NVLLM_BAD_ARGUMENT;
+    try {
+        forget_shared_blocks(pool_k);
+        pools()[pool_k] = PoolInfo{elem_bytes, n_layers, n_kv_heads, head_dim, false};
+    } catch (const std::bad_alloc&) {
+        return NVLLM_NO_MEMORY;
+    }
+    init_free_stack(mgr, block_size, num_blocks);
+    mgr->pool_k = (float*)pool_k;
+    mgr->pool_v = (float*)pool_v;
+    return 0;
 }
 
 }  // extern "C"
-void nvllm::init_block_pool(KVCacheManager* mgr, int block_size, int num_blocks, size_t bytes) {
+void nvllm::init_block_pool(KVCacheManager* mgr, int block_size, int num_blocks, size_t bytes, const std::vector<SlotArrays>& arrays) {
     ensure_init();
     init_free_stack(mgr, block_size, num_blocks);
     void* pool = nullptr;
@@ -390,19 +427,24 @@ void nvllm::init_block_pool(KVCacheManager* mgr, int block_size, int num_blocks,
     HIP_CHECK(hipMemsetAsync(pool, 0, bytes, rt().stream));   // rows nobody has written are finite
     mgr->pool_k = (float*)pool;
     mgr->pool_v = nullptr;
-    block_pools()[pool] = bytes;
+    BlockPool p{bytes, arrays};
+    for (SlotArrays& a : p.arrays) a.base = (char*)pool + (size_t)a.base;
+    block_pools()[pool] = p;
 }
 extern "C" {
 
 void free_kv_cache_manager(KVCacheManager* mgr) {
     if (mgr->free_block_indices) free(mgr->free_block_indices);
     mgr->free_block_indices = nullptr;
+    const auto it = pools().find(mgr->pool_k);
+    const bool owned = it == pools().end() || it->second.owned;
     if (mgr->pool_k) {
-        pools().erase(mgr->pool_k);
+        if (it != pools().end()) pools().erase(it);
         block_pools().erase(mgr->pool_k);
-        device_free(mgr->pool_k);
+        forget_shared_blocks(mgr->pool_k);
+        if (owned) device_free(mgr->pool_k);
     }
-    if (mgr->pool_v) device_free(mgr->pool_v);
+    if (mgr->pool_v && owned) device_free(mgr->pool_v);
     mgr->pool_k = mgr->pool_v = nullptr;
 }
 
@@ -413,6 +455,7 @@ int alloc_block(KVCacheManager* mgr) {
 }
 
 void free_block(KVCacheManager* mgr, int block_idx) {
+    if (drop_shared_block(mgr, block_idx)) return;   // (nvllm_fork_tables: others still use it)
     if (mgr->free_blocks_count >= mgr->num_blocks) return;
     mgr->free_block_indices[mgr->free_blocks_count] = block_idx;
     mgr->free_blocks_count += 1;
@@ -588,7 +631,8 @@ void nvllm_softcap(float* x, float cap, long n) {
 }
 
 void nvllm_latent_pool_init(KVCacheManager* mgr, int block_size, int num_blocks, int rank, int rot, int elem_bytes) {
-    init_block_pool(mgr, block_size, num_blocks, latent_pool_bytes(latent_pool(nullptr, elem_bytes, block_size, rank, rot), num_blocks));
+    const LatentPool p = latent_pool(nullptr, elem_bytes, block_size, rank, rot);
+    init_block_pool(mgr, block_size, num_blocks, latent_pool_bytes(p, num_blocks), {SlotArrays{nullptr, latent_pool_bytes(p, 1), 0, 1}});
 }
 
 static void check_latent_pool(const KVCacheManager* mgr, int rank, int rot, int elem_bytes) {

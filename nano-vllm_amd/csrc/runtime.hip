@@ -218,7 +218,7 @@ static const char* kProfNames[PC_COUNT] = {
     "gemm_other", "rope_kv",  "attn",     "attn_combine", "elementwise", "argmax",    "pack",
     "decode_chain", "gemm_latent_in", "gemm_latent_q", "gemm_absorb", "gemm_value", "latent_kv", "latent_attn", "latent_attn_tok", "latent_combine", "latent_expand", "hyper",
     "conv_rope", "window_attn", "window_attn_tok", "lightning", "lightning_tok", "gemm_router", "route", "expert_rows", "gemm_expert_up", "gemm_expert_down",
-    "gemm_shared_up", "gemm_shared_down", "moe_combine"};
+    "gemm_shared_up", "gemm_shared_down", "moe_combine", "delta", "delta_tok", "slot_copy"};
 
 // --------------------------------------------------------------------- init
 void ensure_init() {

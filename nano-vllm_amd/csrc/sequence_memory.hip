@@ -1,0 +1,383 @@
+// sequence_memory.hip -- copies of blocks and states (sequence_memory.h), and the tables of branching sequences: forks that
+// share whole blocks by count, compaction of a pool, and the release of a table's blocks.
+#include "sequence_memory.h"
+
+#include <algorithm>
+#include <new>
+#include <numeric>
+#include <unordered_map>
+
+namespace nvllm {
+
+bool stream_is_captured() {
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    HIP_CHECK(hipStreamIsCapturing(rt().stream, &st));
+    return st != hipStreamCaptureStatusNone;
+}
+
+// ------------------------------------------------------------------ the copy
+// A program is a list of moves (slot, slot) that a thread makes for its own bytes of a slot, one after the other, in every array
+// alike: no thread touches another's bytes, so programs with different slots need no order, and a cycle of slots is one
+// program with a value set aside (slot -1).  Moves that share a source read it once.
+constexpr int COPY_SETS = 6, COPY_INLINE = 200, COPY_FAN = 4;
+struct CopySet {
+    char* base;
+    size_t stride;
+    unsigned units;   // per slot
+    int first;        // array
+};
+struct CopyArgs {
+    CopySet sets[COPY_SETS];
+    int n_sets, n_programs;
+    const int* programs;          // null: the ints are right here
+    int here[COPY_INLINE];        // [n_programs + 1] first moves, then moves (from, to)
+};
+
+template <typename U, int N>
+__global__ __launch_bounds__(256) void k_copy_slots(CopyArgs a) {
+    const int array = blockIdx.y, program = blockIdx.x % a.n_programs;
+    const unsigned first = (blockIdx.x / a.n_programs) * (256 * N) + threadIdx.x;
+    int set = 0;
+    while (set + 1 < a.n_sets && array >= a.sets[set + 1].first) set++;
+    const unsigned units = a.sets[set].units;
+    if (first >= units) return;
+    U* base = reinterpret_cast<U*>(a.sets[set].base + (size_t)(array - a.sets[set].first) * a.sets[set].stride);
+    const int* prog = a.programs ? a.programs : a.here;
+    const int begin = prog[program], end = prog[program + 1];
+    const int* moves = prog + a.n_programs + 1;
+    U now[N] = {}, aside[N] = {};
+    int have = -2;
+    for (int m = begin; m < end; m++) {
+        const int from = moves[2 * m], to = moves[2 * m + 1];
+        if (from != have) {
+            if (from < 0) {
+#pragma unroll
+                for (int i = 0; i < N; i++) now[i] = aside[i];
+            } else {
+                const U* s = base + (size_t)from * units;
+#pragma unroll
+                for (int i = 0; i < N; i++)
+                    if (first + 256 * i < units) now[i] = s[first + 256 * i];
+            }
+            have = from;
+        }
+        if (to < 0) {
+#pragma unroll
+            for (int i = 0; i < N; i++) aside[i] = now[i];
+        } else {
+            U* d = base + (size_t)to * units;
+#pragma unroll
+            for (int i = 0; i < N; i++)
+                if (first + 256 * i < units) d[first + 256 * i] = now[i];
+        }
+    }
+}
+
+struct Move {
+    int from, to;
+};
+// The moves of a copy as programs: slots that meet are in one, a slot is written after its last reading.  0 or a refusal.
+static int plan_moves(const int* from, const int* to, int n, int n_slots, std::vector<std::vector<Move>>& programs) {
+    std::vector<int> slots;
+    slots.reserve(2 * (size_t)n);
+    for (int i = 0; i < n; i++) {
+        if (from[i] < 0 || from[i] >= n_slots || to[i] < 0 || to[i] >= n_slots) return NVLLM_BAD_INDEX;
+        slots.push_back(from[i]);
+        slots.push_back(to[i]);
+    }
+    std::sort(slots.begin(), slots.end());
+    slots.erase(std::unique(slots.begin(), slots.end()), slots.end());
+    auto at = [&](int s) { return (int)(std::lower_bound(slots.begin(), slots.end(), s) - slots.begin()); };
+    const int k = (int)slots.size();
+    std::vector<int> source(k, -1), uses(k, 0), group(k);
+    std::vector<char> written(k, 0);
+    std::iota(group.begin(), group.end(), 0);
+    auto root = [&](int x) {
+        while (group[x] != x) x = group[x] = group[group[x]];
+        return x;
+    };
+    for (int i = 0; i < n; i++) {
+        const int d = at(to[i]), s = at(from[i]);
+        if (written[d]) return NVLLM_BAD_INDEX;   // two values for one slot
+        written[d] = 1;
+        if (s == d) continue;
+        source[d] = s;
+        uses[s]++;
+        group[root(d)] = root(s);
+    }
+    std::vector<Move> order;
+    std::vector<int> ready;
+    for (int d = 0; d < k; d++)
+        if (source[d] >= 0 && uses[d] == 0) ready.push_back(d);
+    while (!ready.empty()) {
+        const int d = ready.back(), s = source[d];
+        ready.pop_back();
+        order.push_back({s, d});
+        source[d] = -1;
+        if (--uses[s] == 0 && source[s] >= 0) ready.push_back(s);
+    }
+    for (int c = 0; c < k; c++) {
+        if (source[c] < 0) continue;
+        int d = c;
+        order.push_back({c, -1});
+        while (source[d] != c) {
+            order.push_back({source[d], d});
+            const int next = source[d];
+            source[d] = -1;
+            d = next;
+        }
+        order.push_back({-1, d});
+        source[d] = -1;
+    }
+    // by group; a fan out of one source whose slot stays as it is falls into programs of a few moves each
+    std::vector<int> program_of(k, -1);
+    for (const Move& m : order) {
+        const int r = root(m.to >= 0 ? m.to : m.from);
+        if (program_of[r] < 0) {
+            program_of[r] = (int)programs.size();
+            programs.emplace_back();
+        }
+        programs[program_of[r]].push_back({m.from < 0 ? -1 : slots[m.from], m.to < 0 ? -1 : slots[m.to]});
+    }
+    const size_t whole = programs.size();
+    for (size_t p = 0; p < whole; p++) {
+        const std::vector<Move> moves = programs[p];
+        if ((int)moves.size() <= COPY_FAN || std::any_of(moves.begin(), moves.end(), [&](const Move& m) { return m.from != moves[0].from || m.to < 0; })) continue;
+        programs[p].resize(COPY_FAN);
+        for (size_t i = COPY_FAN; i < moves.size(); i += COPY_FAN)
+            programs.emplace_back(moves.begin() + (long)i, moves.begin() + (long)std::min(moves.size(), i + COPY_FAN));
+    }
+    return 0;
+}
+
+template <typename U>
+static void launch_copy(const CopyArgs& a, unsigned most_units, int arrays) {
+    constexpr int N = 2;
+    const long pieces = (most_units + 256 * N - 1) / (256 * N);
+    NVLLM_LAUNCH((k_copy_slots<U, N>), dim3((unsigned)(pieces * a.n_programs), arrays), dim3(256), 0, a);
+}
+
+int copy_slots(const std::vector<SlotArrays>& arrays, int n_slots, const int* from, const int* to, int n) {
+    std::vector<std::vector<Move>> programs;
+    if (const int e = plan_moves(from, to, n, n_slots, programs)) return e;
+    if (programs.empty()) return 0;
+    std::vector<int> ints(programs.size() + 1, 0);
+    for (size_t p = 0; p < programs.size(); p++) ints[p + 1] = ints[p] + (int)programs[p].size();
+    for (const auto& p : programs)
+        for (const Move& m : p) {
+            ints.push_back(m.from);
+            ints.push_back(m.to);
+        }
+    size_t bits = 0;   // of every address and size
+    for (const SlotArrays& s : arrays) {
+        bits |= (size_t)s.base | s.slot_bytes | (s.count > 1 ? s.stride : 0);
+        if (s.count < 0 || s.count > 65535) return NVLLM_BAD_SIZE;
+    }
+    const size_t unit = bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 1;
+    for (const SlotArrays& s : arrays)
+        if (s.slot_bytes / unit > 0x7fffffff || (double)(s.slot_bytes / unit / 512 + 1) * (double)programs.size() > 2e9) return NVLLM_BAD_SIZE;
+    if (ints.size() > staging_ints()) return NVLLM_BAD_SIZE;
+    ensure_init();
+    if (stream_is_captured()) return NVLLM_CAPTURED;
+    CopyArgs a{};
+    a.n_programs = (int)programs.size();
+    if (ints.size() <= COPY_INLINE) {
+        std::copy(ints.begin(), ints.end(), a.here);
+    } else {
+        int* host = pinned_ints((ints.size() + 3) & ~(size_t)3);
+        std::copy(ints.begin(), ints.end(), host);
+        int* dev = (int*)ws_get(WS_STEP, (ints.size() + 4) * sizeof(int));
+        launch_copy_ints(dev, host, ints.size());
+        a.programs = dev;
+    }
+    for (size_t i = 0; i < arrays.size();) {
+        int total = 0;
+        unsigned most = 0;
+        double part = 0;
+        a.n_sets = 0;
+        for (; i < arrays.size() && a.n_sets < COPY_SETS && total + arrays[i].count <= 65535; i++) {
+            const SlotArrays& s = arrays[i];
+            if (s.count == 0 || s.slot_bytes == 0) continue;
+            a.sets[a.n_sets++] = CopySet{(char*)s.base, s.stride, (unsigned)(s.slot_bytes / unit), total};
+            most = std::max(most, (unsigned)(s.slot_bytes / unit));
+            part += 2.0 * n * (double)s.slot_bytes * s.count;
+            total += s.count;
+        }
+        if (total == 0) continue;
+        ProfScope ps(PC_SLOT_COPY, part, 0);
+        if (unit == 16) launch_copy<uint4>(a, most, total);
+        else if (unit == 4) launch_copy<unsigned>(a, most, total);
+        else launch_copy<unsigned char>(a, most, total);
+    }
+    return 0;
+}
+
+// ------------------------------------------------------------------ shared blocks
+// Users of a block beside its first, per pool.  A pool without forks has no entry.
+static std::unordered_map<const void*, std::vector<int>>& shared() {
+    static std::unordered_map<const void*, std::vector<int>> m;
+    return m;
+}
+static int more_users(const KVCacheManager* mgr, int block) {
+    if (shared().empty()) return 0;
+    const auto it = shared().find(mgr->pool_k);
+    return it == shared().end() || block < 0 || block >= (int)it->second.size() ? 0 : it->second[block];
+}
+bool drop_shared_block(const KVCacheManager* mgr, int block) {
+    if (more_users(mgr, block) == 0) return false;
+    shared()[mgr->pool_k][block]--;
+    return true;
+}
+void forget_shared_blocks(const void* pool_k) { shared().erase(pool_k); }
+
+// which blocks lie on the free stack; empty: the stack is not one of this pool
+static std::vector<char> free_blocks(const KVCacheManager* mgr) {
+    std::vector<char> is_free((size_t)mgr->num_blocks, 0);
+    if (mgr->free_blocks_count < 0 || mgr->free_blocks_count > mgr->num_blocks) return {};
+    for (int i = 0; i < mgr->free_blocks_count; i++) {
+        const int b = mgr->free_block_indices[i];
+        if (b < 0 || b >= mgr->num_blocks || is_free[b]) return {};
+        is_free[b] = 1;
+    }
+    return is_free;
+}
+static bool usable(const KVCacheManager* mgr) { return mgr && mgr->free_block_indices && mgr->num_blocks > 0 && mgr->block_size > 0; }
+
+}  // namespace nvllm
+
+using namespace nvllm;
+
+// Every entry point: no exception crosses it, nothing is changed when it refuses.
+#define REFUSING(...)                  \
+    try {                              \
+        __VA_ARGS__                    \
+    } catch (const std::bad_alloc&) {  \
+        return NVLLM_NO_MEMORY;        \
+    }
+
+extern "C" {
+
+int nvllm_copy_states(void* state, size_t slot_bytes, int n_layers, int n_slots, const int* from, const int* to, int n) {
+    if (n < 0 || n_layers < 0 || n_slots < 0 || (n > 0 && (!state || !from || !to))) return NVLLM_BAD_ARGUMENT;
+    if (n == 0 || n_layers == 0 || slot_bytes == 0) return 0;
+    if (slot_bytes > ((size_t)1 << 46) / (size_t)std::max(1, n_slots)) return NVLLM_BAD_SIZE;
+    REFUSING(return copy_slots({SlotArrays{state, slot_bytes, slot_bytes * n_slots, n_layers}}, n_slots, from, to, n);)
+}
+
+int nvllm_copy_blocks(KVCacheManager* mgr, const int* from, const int* to, int n) {
+    if (!usable(mgr) || n < 0 || (n > 0 && (!from || !to))) return NVLLM_BAD_ARGUMENT;
+    if (n == 0) return 0;
+    REFUSING(
+        const std::vector<SlotArrays> arrays = pool_arrays(mgr);
+        if (arrays.empty()) return NVLLM_BAD_SIZE;
+        return copy_slots(arrays, mgr->num_blocks, from, to, n);)
+}
+
+int nvllm_fork_tables(KVCacheManager* mgr, const BlockTable* from, int positions, BlockTable** to, int n) {
+    if (!usable(mgr) || !from || positions < 0 || n < 0 || (n > 0 && !to)) return NVLLM_BAD_ARGUMENT;
+    if (n == 0) return 0;
+    REFUSING(
+        const std::vector<SlotArrays> arrays = pool_arrays(mgr);
+        if (arrays.empty()) return NVLLM_BAD_SIZE;
+        const int whole = positions / mgr->block_size, tail = positions % mgr->block_size != 0;
+        if (from->num_blocks < whole + tail || (whole + tail > 0 && !from->block_indices)) return NVLLM_BAD_INDEX;
+        const std::vector<char> is_free = free_blocks(mgr);
+        if (is_free.empty()) return NVLLM_BAD_INDEX;
+        std::vector<char> seen((size_t)mgr->num_blocks, 0);
+        for (int i = 0; i < whole + tail; i++) {
+            const int b = from->block_indices[i];
+            if (b < 0 || b >= mgr->num_blocks || is_free[b] || seen[b]) return NVLLM_BAD_INDEX;
+            seen[b] = 1;
+        }
+        std::vector<BlockTable*> children(to, to + n);
+        for (BlockTable* t : children)
+            if (!t || t == from || (whole + tail > 0 && !t->block_indices)) return NVLLM_BAD_ARGUMENT;
+        std::sort(children.begin(), children.end());
+        if (std::adjacent_find(children.begin(), children.end()) != children.end()) return NVLLM_BAD_ARGUMENT;
+        if (tail && mgr->free_blocks_count < n) return NVLLM_NO_BLOCKS;
+        std::vector<int> source, target;
+        if (tail) {
+            source.assign((size_t)n, from->block_indices[whole]);
+            for (int i = 0; i < n; i++) target.push_back(mgr->free_block_indices[mgr->free_blocks_count - 1 - i]);
+        }
+        std::vector<int>* users = nullptr;
+        if (whole > 0) {
+            users = &shared()[mgr->pool_k];
+            if ((int)users->size() < mgr->num_blocks) users->resize((size_t)mgr->num_blocks, 0);
+        }
+        if (tail)
+            if (const int e = copy_slots(arrays, mgr->num_blocks, source.data(), target.data(), n)) return e;
+        // (nothing below fails)
+        for (int i = 0; i < whole; i++) (*users)[from->block_indices[i]] += n;
+        for (int i = 0; i < n; i++) {
+            std::copy(from->block_indices, from->block_indices + whole, to[i]->block_indices);
+            if (tail) to[i]->block_indices[whole] = alloc_block(mgr);
+            to[i]->num_blocks = whole + tail;
+        }
+        return 0;)
+}
+
+int nvllm_block_users(const KVCacheManager* mgr, int block) {
+    if (!usable(mgr) || block < 0 || block >= mgr->num_blocks) return NVLLM_BAD_ARGUMENT;
+    for (int i = 0; i < mgr->free_blocks_count; i++)
+        if (mgr->free_block_indices[i] == block) return 0;
+    return 1 + more_users(mgr, block);
+}
+
+int nvllm_free_table(KVCacheManager* mgr, BlockTable* table) {
+    if (!usable(mgr) || !table || table->num_blocks < 0 || (table->num_blocks > 0 && !table->block_indices)) return NVLLM_BAD_ARGUMENT;
+    for (int i = 0; i < table->num_blocks; i++)
+        if (table->block_indices[i] < 0 || table->block_indices[i] >= mgr->num_blocks) return NVLLM_BAD_INDEX;
+    for (; table->num_blocks > 0; table->num_blocks--) free_block(mgr, table->block_indices[table->num_blocks - 1]);
+    return 0;
+}
+
+int nvllm_compact_blocks(KVCacheManager* mgr, BlockTable** tables, int n) {
+    if (!usable(mgr) || n < 0 || (n > 0 && !tables)) return NVLLM_BAD_ARGUMENT;
+    REFUSING(
+        const std::vector<SlotArrays> arrays = pool_arrays(mgr);
+        if (arrays.empty()) return NVLLM_BAD_SIZE;
+        std::vector<char> is_free = free_blocks(mgr);
+        if (is_free.empty()) return NVLLM_BAD_INDEX;
+        // how many of the given tables have a block: one that others use too stays where it is, like one that no table has
+        std::vector<int> found((size_t)mgr->num_blocks, 0);
+        std::vector<BlockTable*> all(tables, tables + n);
+        std::sort(all.begin(), all.end());
+        if (std::adjacent_find(all.begin(), all.end()) != all.end()) return NVLLM_BAD_ARGUMENT;
+        for (const BlockTable* t : all) {
+            if (!t || t->num_blocks < 0 || (t->num_blocks > 0 && !t->block_indices)) return NVLLM_BAD_ARGUMENT;
+            for (int i = 0; i < t->num_blocks; i++) {
+                const int b = t->block_indices[i];
+                if (b < 0 || b >= mgr->num_blocks || is_free[b]) return NVLLM_BAD_INDEX;
+                found[b]++;
+            }
+        }
+        const int used = mgr->num_blocks - mgr->free_blocks_count;
+        std::vector<int> from, to, place((size_t)mgr->num_blocks);
+        std::iota(place.begin(), place.end(), 0);
+        int hole = 0;
+        for (int b = used; b < mgr->num_blocks; b++) {
+            if (is_free[b] || found[b] == 0 || found[b] < 1 + more_users(mgr, b)) continue;
+            while (!is_free[hole]) hole++;   // (there are as many below `used` as blocks in use behind it)
+            from.push_back(b);
+            to.push_back(hole);
+            place[b] = hole++;
+        }
+        if (!from.empty())
+            if (const int e = copy_slots(arrays, mgr->num_blocks, from.data(), to.data(), (int)from.size())) return e;
+        // (nothing below fails)
+        const auto users = shared().find(mgr->pool_k);
+        for (size_t i = 0; i < from.size(); i++) {
+            is_free[from[i]] = 1;
+            is_free[to[i]] = 0;
+            if (users != shared().end()) std::swap(users->second[from[i]], users->second[to[i]]);
+        }
+        for (BlockTable* t : all)
+            for (int i = 0; i < t->num_blocks; i++) t->block_indices[i] = place[t->block_indices[i]];
+        int count = 0;
+        for (int b = mgr->num_blocks - 1; b >= 0; b--)
+            if (is_free[b]) mgr->free_block_indices[count++] = b;
+        return (int)from.size();)
+}
+
+}  // extern "C"

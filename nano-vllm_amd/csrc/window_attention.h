@@ -4,6 +4,7 @@
 #pragma once
 
 #include "nvllm_internal.h"
+#include "sequence_memory.h"
 #include "step_arrays.h"
 
 namespace nvllm {
@@ -24,6 +25,8 @@ struct KvPages {
 constexpr int KV_PAGE = 16;
 KvPages kv_pages(void* base, int elem_bytes, int block_size, int num_blocks, int G, int dim, int vdim);
 size_t kv_pages_bytes(int elem_bytes, int block_size, int num_blocks, int G, int dim, int vdim);
+// where the blocks of a slice that begins at `offset` lie: of the keys, of the values
+void add_kv_pages(std::vector<SlotArrays>& to, size_t offset, int elem_bytes, int block_size, int num_blocks, int G, int dim, int vdim);
 
 // Convolution, rotation and cache write of a batch's projected rows.
 struct ConvRope {

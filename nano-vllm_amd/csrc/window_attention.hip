@@ -37,6 +37,13 @@ size_t kv_pages_bytes(int elem_bytes, int block_size, int num_blocks, int G, int
     return ((size_t)num_blocks * block_size * G * (p.dim_ld + p.vdim_ld) * elem_bytes + 255) & ~(size_t)255;
 }
 
+void add_kv_pages(std::vector<SlotArrays>& to, size_t offset, int elem_bytes, int block_size, int num_blocks, int G, int dim, int vdim) {
+    const KvPages p = kv_pages(nullptr, elem_bytes, block_size, num_blocks, G, dim, vdim);
+    const size_t rows = (size_t)block_size * G * elem_bytes;
+    to.push_back(SlotArrays{(void*)offset, rows * p.dim_ld, 0, 1});
+    to.push_back(SlotArrays{(void*)(offset + rows * num_blocks * p.dim_ld), rows * p.vdim_ld, 0, 1});
+}
+
 // accumulators of k_window_attn_any: a set per group of threads, or one row that is wider than the workgroup
 __host__ __device__ inline int window_any_acc(int vdim_ld, int vec) { return vdim_ld > 256 * vec ? vdim_ld : 256 * vec; }
 __device__ __forceinline__ float b16_f32(unsigned short v) { return __builtin_bit_cast(float, (unsigned)v << 16); }
