@@ -17,9 +17,25 @@ struct Delta {
     long q_ld, k_ld, v_ld;
     float scale, eps;           // eps 0: queries and keys as they are
     int Q, H, dim, vdim;
+    int dim_kept;               // of the state: dim without padding
     const int4* spans;          // (first token, count, first position, slot); null: the ones here
     int n_spans;
     int4 here[DELTA_SPANS];
+};
+
+// Portions of several tokens in chunks of DELTA_CHUNK tokens.
+constexpr int DELTA_CHUNK = 64;
+// What a chunk's tokens need of each other, per (chunk, head): the operands of T' and P (six 16 x 32 tiles on and below the diagonal
+// each, three parts), then per token the factors a, b and c, then what is left of the state.
+constexpr int DELTA_PART = 1024, DELTA_TILE = 3 * DELTA_PART, DELTA_OPS = 12 * DELTA_TILE, DELTA_RECORD = DELTA_OPS + 1024;
+struct DeltaChunks {
+    Delta a;                    // queries and keys: dims padded with zeros to a multiple of 8, rows 16-byte aligned
+    char* mem;                  // [chunk of the launch][H] records
+    const int* first;           // [n_spans] the launch's first chunk of each span; null: the ones here
+    int first_here[DELTA_SPANS];
+    int from, most;             // chunks [from, from + most) of every span
+    bool out_four;              // out can be stored four elements at a time
+    double bytes, flops;        // kernel timing
 };
 
 }  // namespace nvllm

@@ -4,6 +4,14 @@
 //   u = beta (v - e^g a),   o = scale (e^g b + c u),   S <- e^g S + k u^T,
 // so one pass over S and one sum over its rows serve both.  A wave holds 32 value columns of a head's state in registers (a lane: 4
 // columns x NR rows), reads it once, goes through the portion's tokens and writes it once.
+//
+// Portions of several tokens go in chunks of 64.  With G_t the sum of g up to token t of the chunk, k and q normed, S the state in front:
+//   A_ts = beta_t e^(G_t - G_s) k_t . k_s  for s < t,   T' = (I + A)^-1 diag(beta),   P_ts = scale e^(G_t - G_s) q_t . k_s  for s <= t,
+//   X_t = v_t - e^(G_t) S^T k_t,   U = T' X,   o_t = scale e^(G_t) S^T q_t + sum_s P_ts u_s,   S <- e^(G_n) S + sum_s e^(G_n - G_s) k_s u_s^T
+// k_delta_prepare forms T' and P of all chunks and heads side by side, k_delta_chunks walks a portion's chunks.  What norms keys and
+// queries is a factor per token, so the rows themselves enter the matrix cores as they are: bf16 values exactly.  All other
+// factors (S, X, U, T', P, and fp32 rows) enter as three bf16 parts, 26 bits together: a product of two of them is the six products
+// of parts above 2^-26.
 #include "gated_delta.h"
 
 #include <algorithm>
@@ -178,6 +186,507 @@ static void launch_step(const Delta& a) {
     else NVLLM_LAUNCH((k_delta_step<B16, 32, VEC>), grid, dim3(64), 0, a);
 }
 
+// ------------------------------------------------------------------ chunks
+typedef short s4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s4_t lds_s4;
+constexpr int CH = DELTA_CHUNK;
+constexpr float MIN_G = -1e4f;   // e^MIN_G is zero, and differences of sums of it are numbers
+
+// x = a + b + c, each rounded to the nearest bf16 of what is left: exact but for the 26th bit, and what a product of two leaves out has no
+// sign of its own.  (Truncations, of the factors' own signs, left a bias: sums of 64 corrections to one key were off by 520 halves
+// of a step.)
+__device__ __forceinline__ unsigned two_b16(float lo, float hi) {
+    typedef __bf16 b2_t __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(unsigned, b2_t{(__bf16)lo, (__bf16)hi});
+}
+__device__ __forceinline__ void parts_of_four(const f4_t& v, u2_t (&out)[3]) {
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        float lo = v[2 * i], hi = v[2 * i + 1];
+#pragma unroll
+        for (int k = 0; k < 3; k++) {
+            const unsigned p = two_b16(lo, hi);
+            out[k][i] = p;
+            lo -= __builtin_bit_cast(float, p << 16);
+            hi -= __builtin_bit_cast(float, p & 0xffff0000u);
+        }
+    }
+}
+__device__ __forceinline__ void parts_of_eight(const f4_t& lo, const f4_t& hi, b8_t (&out)[3]) {
+    u2_t l[3], h[3];
+    parts_of_four(lo, l);
+    parts_of_four(hi, h);
+#pragma unroll
+    for (int k = 0; k < 3; k++) out[k] = __builtin_bit_cast(b8_t, u4_t{l[k][0], l[k][1], h[k][0], h[k][1]});
+}
+__device__ __forceinline__ f4_t mfma(const b8_t& a, const b8_t& b, const f4_t& c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+// the six products of 32-bit values' parts, small ones first
+__device__ __forceinline__ f4_t mfma6(const b8_t (&a)[3], const b8_t (&b)[3], f4_t c) {
+    c = mfma(a[1], b[1], c);
+    c = mfma(a[2], b[0], c);
+    c = mfma(a[0], b[2], c);
+    c = mfma(a[1], b[0], c);
+    c = mfma(a[0], b[1], c);
+    return mfma(a[0], b[0], c);
+}
+__device__ __forceinline__ f4_t mfma4(float a, float b, const f4_t& c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ float exp_of(double x) { return __builtin_amdgcn_exp2f((float)(x * 1.4426950408889634)); }
+
+// A token's row of queries or keys as operands: lane (x, g) has dims 32 cc + 8 g .. + 7 of the tile's row x.
+template <int DC, bool B16>
+struct Rows {
+    static constexpr int W = B16 ? 1 : 2;
+    u4_t w[DC][W];
+    __device__ __forceinline__ void load(const void* base, size_t row, int dim, int g, bool there) {
+#pragma unroll
+        for (int cc = 0; cc < DC; cc++) {
+            const int d = 32 * cc + 8 * g;
+#pragma unroll
+            for (int i = 0; i < W; i++) {
+                w[cc][i] = u4_t{0, 0, 0, 0};
+                if (there && d < dim) w[cc][i] = *reinterpret_cast<const u4_t*>((const char*)base + (row + d) * (B16 ? 2 : 4) + 16 * i);
+            }
+        }
+    }
+    __device__ __forceinline__ void operand(int cc, b8_t (&p)[B16 ? 1 : 3]) const {
+        if constexpr (B16) p[0] = __builtin_bit_cast(b8_t, w[cc][0]);
+        else parts_of_eight(__builtin_bit_cast(f4_t, w[cc][0]), __builtin_bit_cast(f4_t, w[cc][1]), p);
+    }
+    __device__ __forceinline__ float squares() const {   // of this lane's values
+        float s = 0.f;
+#pragma unroll
+        for (int cc = 0; cc < DC; cc++)
+#pragma unroll
+            for (int i = 0; i < W; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const unsigned bits = w[cc][i][e];   // (a value: the cast of a vector's element in place takes the first one)
+                    if (B16) {
+                        const float lo = __builtin_bit_cast(float, bits << 16), hi = __builtin_bit_cast(float, bits & 0xffff0000u);
+                        s = fmaf(lo, lo, fmaf(hi, hi, s));
+                    } else {
+                        const float v = __builtin_bit_cast(float, bits);
+                        s = fmaf(v, v, s);
+                    }
+                }
+        return s;
+    }
+};
+// products over all dims: rows of a, columns of b
+template <bool B16>
+__device__ __forceinline__ f4_t mfma_rows(const b8_t (&a)[B16 ? 1 : 3], const b8_t (&b)[B16 ? 1 : 3], f4_t c) {
+    if constexpr (B16) return mfma(a[0], b[0], c);
+    else return mfma6(a, b, c);
+}
+
+struct ChunkAt {
+    int4 span;
+    int first, n;   // token of the batch, tokens
+    char* record;
+};
+__device__ __forceinline__ ChunkAt chunk_at(const DeltaChunks& c, int s, int h, int i) {
+    ChunkAt at;
+    at.span = (c.a.spans ? c.a.spans : c.a.here)[s];
+    at.first = at.span.x + (c.from + i) * CH;
+    at.n = min(CH, at.span.y - (c.from + i) * CH);
+    at.record = c.mem + ((size_t)((c.first ? c.first : c.first_here)[s] + i) * c.a.H + h) * DELTA_RECORD;
+    return at;
+}
+// T' and P: tile (token tile w, 32 tokens p) of the six that are not empty
+__device__ __forceinline__ int op_tile(int w, int p) { return w < 2 ? w : 2 * w - 2 + p; }
+
+constexpr int LD = CH + 4;   // floats of a row of A or T in LDS
+template <int DC, bool B16>
+constexpr int prepare_lds() { return 4 * DC * (B16 ? 1 : 3) * 1024 + 2 * CH * LD * 4 + CH * (8 + 4 + 4); }
+
+template <int DC, bool B16>
+__global__ __launch_bounds__(256) void k_delta_prepare(DeltaChunks c) {
+    constexpr int PARTS = B16 ? 1 : 3;
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds_d[];
+    u4_t* s_k = reinterpret_cast<u4_t*>(lds_d);                            // [token tile][DC][part][64]
+    float* s_A = reinterpret_cast<float*>(s_k + 4 * DC * PARTS * 64);      // [t][LD]
+    float* s_T = s_A + CH * LD;
+    double* s_G = reinterpret_cast<double*>(s_T + CH * LD);
+    float* s_r = reinterpret_cast<float*>(s_G + CH);                       // what norms a key
+    float* s_b = s_r + CH;
+    const Delta& a = c.a;
+    const int h = blockIdx.x, hq = h / (a.H / a.Q);
+    const ChunkAt at = chunk_at(c, blockIdx.z, h, blockIdx.y);
+    if (at.n <= 0) return;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), x = lane & 15, g = lane >> 4;
+    const int t = 16 * w + x;
+    Rows<DC, B16> k, q;
+    const bool there = t < at.n;
+    k.load(a.k, (size_t)(at.first + t) * a.k_ld + hq * a.dim, a.dim, g, there);
+    q.load(a.q, (size_t)(at.first + t) * a.q_ld + hq * a.dim, a.dim, g, there);
+    if (w == 0) {
+        const size_t i = (size_t)(at.first + min(lane, at.n - 1)) * a.H + h;
+        const float gl = a.g[i];
+        double G = lane < at.n ? (double)(gl < MIN_G ? MIN_G : gl) : 0.0;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const double before = __shfl_up(G, o, 64);
+            if (lane >= o) G += before;
+        }
+        s_G[lane] = G;
+        s_b[lane] = lane < at.n ? a.beta[i] : 0.f;
+    }
+    float rk = 1.f, rq = 1.f;
+    if (a.eps > 0.f) {
+        float kk = k.squares(), qq = q.squares();
+        kk += __shfl_xor(kk, 16, 64);
+        qq += __shfl_xor(qq, 16, 64);
+        kk += __shfl_xor(kk, 32, 64);
+        qq += __shfl_xor(qq, 32, 64);
+        rk = 1.f / sqrtf(kk + a.eps);
+        rq = 1.f / sqrtf(qq + a.eps);
+    }
+    if (g == 0) s_r[t] = rk;
+    b8_t ko[DC][PARTS], qo[DC][PARTS];
+#pragma unroll
+    for (int cc = 0; cc < DC; cc++) {
+        k.operand(cc, ko[cc]);
+        q.operand(cc, qo[cc]);
+#pragma unroll
+        for (int p = 0; p < PARTS; p++) s_k[((w * DC + cc) * PARTS + p) * 64 + lane] = __builtin_bit_cast(u4_t, ko[cc][p]);
+    }
+    __syncthreads();
+    // rows s of tile i, columns t of tile w
+    const double Gt = s_G[t];
+    const float bt = s_b[t] * rk, qt = a.scale * rq;
+    f4_t kq[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        f4_t kk = {0.f, 0.f, 0.f, 0.f};
+        kq[i] = f4_t{0.f, 0.f, 0.f, 0.f};
+        if (i <= w) {
+#pragma unroll
+            for (int cc = 0; cc < DC; cc++) {
+                b8_t r[PARTS];
+#pragma unroll
+                for (int p = 0; p < PARTS; p++) r[p] = __builtin_bit_cast(b8_t, s_k[((i * DC + cc) * PARTS + p) * 64 + lane]);
+                kk = mfma_rows<B16>(r, ko[cc], kk);
+                kq[i] = mfma_rows<B16>(r, qo[cc], kq[i]);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int s = 16 * i + 4 * g + r;
+                const float f = exp_of(Gt - s_G[s]) * s_r[s];   // (not used where s lies behind t)
+                kk[r] = s < t ? bt * f * kk[r] : 0.f;
+                kq[i][r] = s <= t ? qt * f * kq[i][r] : 0.f;
+            }
+        }
+        *reinterpret_cast<f4_t*>(s_A + t * LD + 16 * i + 4 * g) = kk;
+    }
+    u4_t* ops = reinterpret_cast<u4_t*>(at.record) + lane;
+#pragma unroll
+    for (int p = 0; p < 2; p++)
+        if (p <= w >> 1) {
+            b8_t parts[3];
+            parts_of_eight(kq[2 * p], kq[2 * p + 1], parts);
+#pragma unroll
+            for (int j = 0; j < 3; j++) ops[((6 + op_tile(w, p)) * 3 + j) * 64] = __builtin_bit_cast(u4_t, parts[j]);
+        }
+    if (threadIdx.x < CH) {   // (wave 0: t is not this thread's token)
+        float* f = reinterpret_cast<float*>(at.record + DELTA_OPS);
+        const int tok = threadIdx.x;
+        f[tok] = exp_of(s_G[tok]) * s_r[tok];
+        f[2 * CH + tok] = exp_of(s_G[CH - 1] - s_G[tok]) * s_r[tok];
+        if (tok == 0) f[3 * CH] = exp_of(s_G[CH - 1]);
+    }
+    if (g == 0) reinterpret_cast<float*>(at.record + DELTA_OPS)[CH + t] = qt * exp_of(Gt);
+    __syncthreads();
+    // (I + A)^-1: wave w first its block on the diagonal, a lane a column ...
+    {
+        float col[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            float v = i == x ? 1.f : 0.f;
+#pragma unroll
+            for (int s4 = 0; s4 < (i + 3) / 4; s4++) {
+                const f4_t A = *reinterpret_cast<const f4_t*>(s_A + (16 * w + i) * LD + 16 * w + 4 * s4);
+#pragma unroll
+                for (int s = 4 * s4; s < i && s < 4 * s4 + 4; s++) v = fmaf(-A[s & 3], col[s], v);
+            }
+            col[i] = v;
+        }
+        if (g == 0)
+#pragma unroll
+            for (int i = 0; i < 16; i++) s_T[(16 * w + i) * LD + 16 * w + x] = col[i];
+    }
+    __syncthreads();
+    // ... then the blocks under it, from the top: T_iw = -T_ii sum_j A_ij T_jw.  (k of these products runs 4 g + step, as results lie)
+    {
+        f4_t T[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++) T[0][r] = s_T[(16 * w + 4 * g + r) * LD + 16 * w + x];
+#pragma unroll
+        for (int j = 1; j < 4; j++) {
+            const int i = w + j;
+            if (i >= 4) break;
+            f4_t sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int m = 0; m < j; m++) {
+                const f4_t A = *reinterpret_cast<const f4_t*>(s_A + (16 * i + x) * LD + 16 * (w + m) + 4 * g);
+#pragma unroll
+                for (int e = 0; e < 4; e++) sum = mfma4(A[e], T[m][e], sum);
+            }
+            const f4_t D = *reinterpret_cast<const f4_t*>(s_T + (16 * i + x) * LD + 16 * i + 4 * g);
+            T[j] = f4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int e = 0; e < 4; e++) T[j] = mfma4(-D[e], sum[e], T[j]);
+#pragma unroll
+            for (int r = 0; r < 4; r++) s_T[(16 * i + 4 * g + r) * LD + 16 * w + x] = T[j][r];
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int p = 0; p < 2; p++)
+        if (p <= w >> 1) {
+            f4_t v[2];
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+                const int s0 = 32 * p + 16 * half + 4 * g;
+                v[half] = f4_t{0.f, 0.f, 0.f, 0.f};
+                if (2 * p + half <= w) v[half] = *reinterpret_cast<const f4_t*>(s_T + t * LD + s0);
+#pragma unroll
+                for (int r = 0; r < 4; r++) v[half][r] = v[half][r] * s_b[s0 + r];
+            }
+            b8_t parts[3];
+            parts_of_eight(v[0], v[1], parts);
+#pragma unroll
+            for (int j = 0; j < 3; j++) ops[(op_tile(w, p) * 3 + j) * 64] = __builtin_bit_cast(u4_t, parts[j]);
+        }
+}
+
+// A workgroup = (portion, head, 16 value columns); wave w has tokens 16 w .. + 15 of a chunk and the state's dim tiles w, w + 4, ..
+// A dim tile's row 4 g + r is dim 32 (i / 2) + 8 g + 4 (i & 1) + r, so that a lane's eight values of two tiles are the k of one
+// operand and a row's 16 bytes of keys are the other.
+template <int DC, bool B16>
+constexpr int chunks_lds() { return (3 * DC + 6 + 6 + 6) * 1024 + (B16 ? 1 : 3) * CH * (32 * DC + 8) * 2; }
+
+template <int DC, bool B16>
+__global__ __launch_bounds__(256) void k_delta_chunks(DeltaChunks c) {
+    constexpr int PARTS = B16 ? 1 : 3, TILES = (2 * DC + 3) / 4, ROW = 32 * DC + 8;
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds_d[];
+    u4_t* s_S = reinterpret_cast<u4_t*>(lds_d);   // [DC][part][64]
+    u4_t* s_X = s_S + DC * 3 * 64;                // [32 tokens][part][64]
+    u4_t* s_U = s_X + 6 * 64;
+    u4_t* s_V = s_U + 6 * 64;                     // U as the state takes it
+    unsigned short* s_k = reinterpret_cast<unsigned short*>(s_V + 6 * 64);   // [part][token][ROW]
+    const Delta& a = c.a;
+    const int h = blockIdx.x, slice = blockIdx.y, hq = h / (a.H / a.Q);
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), x = lane & 15, g = lane >> 4;
+    const int4 span = (a.spans ? a.spans : a.here)[blockIdx.z];
+    const int chunks = min(c.most, (span.y + CH - 1) / CH - c.from);
+    if (chunks <= 0) return;
+    const int col = slice * 16 + x;   // of the state, of V
+    const bool has_col = col < a.vdim, upper = w >= 2;
+    float* st = a.state + ((size_t)span.w * a.H + h) * a.dim_kept * a.vdim;
+    // ---- the state: this wave's tiles, and all of them as operands
+    f4_t S[TILES];
+    auto dim_of = [&](int i) { return 32 * (i >> 1) + 8 * g + 4 * (i & 1); };
+#pragma unroll
+    for (int j = 0; j < TILES; j++) {
+        const int i = w + 4 * j, d0 = dim_of(i);
+#pragma unroll
+        for (int r = 0; r < 4; r++) S[j][r] = span.z + c.from > 0 && has_col && i < 2 * DC && d0 + r < a.dim_kept ? st[(size_t)(d0 + r) * a.vdim + col] : 0.f;
+    }
+    auto put = [&](u4_t* to, int half, const f4_t& v) {   // [part][64] operands: one half of a lane's eight values
+        u2_t parts[3];
+        parts_of_four(v, parts);
+#pragma unroll
+        for (int p = 0; p < 3; p++) reinterpret_cast<u2_t*>(to + p * 64 + lane)[half] = parts[p];
+    };
+    auto get = [&](const u4_t* from, b8_t (&p)[3]) {
+#pragma unroll
+        for (int j = 0; j < 3; j++) p[j] = __builtin_bit_cast(b8_t, from[j * 64 + lane]);
+    };
+    auto put_state = [&] {
+#pragma unroll
+        for (int j = 0; j < TILES; j++)
+            if (w + 4 * j < 2 * DC) put(s_S + ((w + 4 * j) >> 1) * 3 * 64, w & 1, S[j]);
+    };
+    put_state();
+    // ---- a chunk's rows, factors and operands, each asked for when the last chunk's are used
+    Rows<DC, B16> k, q;
+    float v[4], fb, fade;
+    f4_t fa, fc;
+    b8_t to[2][3], po[2][3];
+    auto fetch_rows = [&](int i) {
+        const ChunkAt at = chunk_at(c, blockIdx.z, h, i);
+        const int t = 16 * w + x;
+        k.load(a.k, (size_t)(at.first + t) * a.k_ld + hq * a.dim, a.dim, g, t < at.n);
+        q.load(a.q, (size_t)(at.first + t) * a.q_ld + hq * a.dim, a.dim, g, t < at.n);
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const int tok = 16 * w + 4 * g + r;
+            v[r] = 0.f;
+            if (tok < at.n && has_col) {
+                const size_t e = (size_t)(at.first + tok) * a.v_ld + h * a.vdim + col;
+                v[r] = B16 ? __builtin_bit_cast(float, (unsigned)((const unsigned short*)a.v)[e] << 16) : ((const float*)a.v)[e];
+            }
+        }
+        const float* f = reinterpret_cast<const float*>(at.record + DELTA_OPS);
+        fa = *reinterpret_cast<const f4_t*>(f + 16 * w + 4 * g);
+        fb = f[CH + t];
+    };
+    auto fetch_ops = [&](int i, int what, b8_t (&o)[2][3]) {
+        const u4_t* ops = reinterpret_cast<const u4_t*>(chunk_at(c, blockIdx.z, h, i).record) + lane;
+#pragma unroll
+        for (int p = 0; p < 2; p++)
+#pragma unroll
+            for (int j = 0; j < 3; j++) {
+                o[p][j] = b8_t{};
+                if (p == 0 || upper) o[p][j] = __builtin_bit_cast(b8_t, ops[((what * 6 + op_tile(w, p)) * 3 + j) * 64]);
+            }
+    };
+    auto fetch_factors = [&](int i) {
+        const float* f = reinterpret_cast<const float*>(chunk_at(c, blockIdx.z, h, i).record + DELTA_OPS);
+        fc = *reinterpret_cast<const f4_t*>(f + 2 * CH + 16 * w + 4 * g);
+        fade = f[3 * CH];
+    };
+    fetch_rows(0);
+    fetch_ops(0, 0, to);
+    fetch_factors(0);
+    fetch_ops(0, 1, po);
+    __syncthreads();
+    for (int i = 0; i < chunks; i++) {
+        const ChunkAt at = chunk_at(c, blockIdx.z, h, i);
+        const int next = min(i + 1, chunks - 1);
+        // ---- S^T k and S^T q
+        f4_t D[2] = {}, O[2] = {};
+#pragma unroll
+        for (int cc = 0; cc < DC; cc++) {
+            b8_t s[3], kp[PARTS], qp[PARTS];
+            get(s_S + cc * 3 * 64, s);
+            k.operand(cc, kp);
+            q.operand(cc, qp);
+#pragma unroll
+            for (int p = 0; p < PARTS; p++) *reinterpret_cast<u4_t*>(s_k + (p * CH + 16 * w + x) * ROW + 32 * cc + 8 * g) = __builtin_bit_cast(u4_t, kp[p]);
+            if constexpr (B16) {
+#pragma unroll
+                for (int p = 2; p >= 0; p--) {
+                    D[p & 1] = mfma(kp[0], s[p], D[p & 1]);
+                    O[p & 1] = mfma(s[p], qp[0], O[p & 1]);
+                }
+            } else {
+                D[cc & 1] = mfma6(kp, s, D[cc & 1]);
+                O[cc & 1] = mfma6(s, qp, O[cc & 1]);
+            }
+        }
+        f4_t X;
+        const f4_t d = D[0] + D[1];
+#pragma unroll
+        for (int r = 0; r < 4; r++) X[r] = fmaf(-fa[r], d[r], v[r]);
+        f4_t o = (O[0] + O[1]) * fb;
+        put(s_X + (w >> 1) * 3 * 64, w & 1, X);
+        fetch_rows(next);
+        __syncthreads();
+        // ---- U = T' X
+        f4_t U = {0.f, 0.f, 0.f, 0.f};
+        b8_t e[3];
+        get(s_X, e);
+        U = mfma6(to[0], e, U);
+        if (upper) {
+            get(s_X + 3 * 64, e);
+            U = mfma6(to[1], e, U);
+        }
+        put(s_U + (w >> 1) * 3 * 64, w & 1, U);
+        put(s_V + (w >> 1) * 3 * 64, w & 1, U * fc);
+        const float left = fade;
+        fetch_ops(next, 0, to);
+        fetch_factors(next);
+        __syncthreads();
+        // ---- the state: keys as columns from LDS (16 lanes bring 4 tokens x 16 dims, lane x receives dim x of the four)
+        b8_t u[2][3];
+        get(s_V, u[0]);
+        get(s_V + 3 * 64, u[1]);
+#pragma unroll
+        for (int j = 0; j < TILES; j++) {
+            const int tile = w + 4 * j;
+            if (tile >= 2 * DC) break;
+            S[j] *= left;
+#pragma unroll
+            for (int p = 0; p < 2; p++) {
+                b8_t kt[PARTS];
+#pragma unroll
+                for (int part = 0; part < PARTS; part++) {
+                    const unsigned short* at_k = s_k + (part * CH + 32 * p + 4 * g + (x >> 2)) * ROW + 32 * (tile >> 1) + 8 * (x & 3) + 4 * (tile & 1);
+                    const u2_t lo = __builtin_bit_cast(u2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)at_k));
+                    const u2_t hi = __builtin_bit_cast(u2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at_k + 16 * ROW)));
+                    kt[part] = __builtin_bit_cast(b8_t, u4_t{lo[0], lo[1], hi[0], hi[1]});
+                }
+                if constexpr (B16) {
+#pragma unroll
+                    for (int part = 2; part >= 0; part--) S[j] = mfma(kt[0], u[p][part], S[j]);
+                } else S[j] = mfma6(kt, u[p], S[j]);
+            }
+        }
+        put_state();
+        // ---- the results: lane (x, g) has token 16 w + x, columns 4 g .. + 3
+        get(s_U, e);
+        o = mfma6(e, po[0], o);
+        if (upper) {
+            get(s_U + 3 * 64, e);
+            o = mfma6(e, po[1], o);
+        }
+        fetch_ops(next, 1, po);
+        if (16 * w + x < at.n) {
+            const int oc = slice * 16 + 4 * g;
+            const size_t e0 = ((size_t)(at.first + 16 * w + x) * a.H + h) * a.vdim + oc;
+            if (c.out_four) store_four<B16, true>(a.out, e0, o, a.vdim - oc);
+            else store_four<B16, false>(a.out, e0, o, a.vdim - oc);
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int j = 0; j < TILES; j++) {
+        const int i = w + 4 * j, d0 = dim_of(i);
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+            if (has_col && i < 2 * DC && d0 + r < a.dim_kept) st[(size_t)(d0 + r) * a.vdim + col] = S[j][r];
+    }
+}
+
+// Rows of queries and keys whose dims or addresses the chunk kernels' loads do not fit: dims padded to a multiple of 8 with zeros.
+template <typename E>
+__global__ __launch_bounds__(256) void k_delta_rows(E* __restrict__ dst, const E* __restrict__ src, int Q, int dim, int dim_ld, long ld) {
+    const long row = blockIdx.x;
+    for (int i = threadIdx.x; i < Q * dim_ld; i += 256) {
+        const int hq = i / dim_ld, d = i - hq * dim_ld;
+        dst[row * Q * dim_ld + i] = d < dim ? src[row * ld + hq * dim + d] : (E)0;
+    }
+}
+
+template <int DC, bool B16>
+static void launch_chunks_of(const DeltaChunks& c) {
+    const Delta& a = c.a;
+    constexpr int prep = prepare_lds<DC, B16>(), walk = chunks_lds<DC, B16>();
+    static bool enabled = false;
+    if (!enabled) {
+        HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(&k_delta_prepare<DC, B16>), hipFuncAttributeMaxDynamicSharedMemorySize, prep));
+        HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(&k_delta_chunks<DC, B16>), hipFuncAttributeMaxDynamicSharedMemorySize, walk));
+        enabled = true;
+    }
+    {
+        ProfScope ps(PC_DELTA, c.bytes / 2, c.flops / 2);
+        NVLLM_LAUNCH((k_delta_prepare<DC, B16>), dim3(a.H, c.most, a.n_spans), dim3(256), prep, c);
+    }
+    ProfScope ps(PC_DELTA, c.bytes / 2, c.flops / 2);
+    NVLLM_LAUNCH((k_delta_chunks<DC, B16>), dim3(a.H, cdiv(a.vdim, 16), a.n_spans), dim3(256), walk, c);
+}
+template <bool B16>
+static void launch_chunks(const DeltaChunks& c) {
+    const int steps = cdiv(c.a.dim, 32);
+    if (steps == 1) launch_chunks_of<1, B16>(c);
+    else if (steps == 2) launch_chunks_of<2, B16>(c);
+    else if (steps == 3) launch_chunks_of<3, B16>(c);
+    else if (steps == 4) launch_chunks_of<4, B16>(c);
+    else if (steps <= 6) launch_chunks_of<6, B16>(c);
+    else launch_chunks_of<8, B16>(c);
+}
+
 // Portions of a batch; a refusal if its sequences do not fit.
 static int delta_spans(std::vector<int4>& spans, const int* seq_ids, const int* pos, int T, int n_slots) {
     for (int t = 0; t < T;) {
@@ -196,30 +705,111 @@ static int delta_spans(std::vector<int4>& spans, const int* seq_ids, const int* 
     return std::adjacent_find(ids.begin(), ids.end()) == ids.end() ? 0 : NVLLM_BAD_INDEX;
 }
 
+// Where a batch's portions go: the first n_chunked by chunks, the others token by token.
+constexpr int CHUNK_MIN = 16;                          // tokens of a portion that goes by chunks
+constexpr size_t CHUNK_MEMORY = (size_t)192 << 20;     // of the chunks' records at a time
+
 static int gated_delta(Delta& a, const int* seq_ids, const int* pos, int T, int n_slots, int elem) {
     std::vector<int4> spans;
     if (const int e = delta_spans(spans, seq_ids, pos, T, n_slots)) return e;
-    if ((double)cdiv(a.vdim, STEP_COLS) * a.H * (double)spans.size() > 2e9 || spans.size() * 4 > staging_ints()) return NVLLM_BAD_SIZE;
+    if ((double)cdiv(a.vdim, STEP_COLS) * a.H * (double)spans.size() > 2e9) return NVLLM_BAD_SIZE;
+    const bool b16 = elem == 2;
+    std::stable_sort(spans.begin(), spans.end(), [](const int4& l, const int4& r) { return (l.y >= CHUNK_MIN) > (r.y >= CHUNK_MIN); });
+    int n_chunked = 0, longest = 0;
+    long tokens = 0;
+    double states[2] = {0, 0};
+    for (const int4& s : spans) {
+        const bool ch = s.y >= CHUNK_MIN;
+        states[ch] += (s.z > 0 ? 8.0 : 4.0) * a.H * a.dim * (double)a.vdim;
+        if (!ch) continue;
+        n_chunked++;
+        tokens += s.y;
+        longest = std::max(longest, cdiv(s.y, CH));
+    }
+    // chunks of every portion per launch, and each portion's first record then
+    int most = 0;
+    std::vector<int> first(spans.size(), 0);
+    if (n_chunked > 0) {
+        const size_t room = std::max((size_t)1, CHUNK_MEMORY / ((size_t)a.H * DELTA_RECORD));
+        auto records = [&](int per) {
+            size_t n = 0;
+            for (int i = 0; i < n_chunked; i++) {
+                first[i] = (int)n;
+                n += (size_t)std::min(per, cdiv(spans[i].y, CH));
+            }
+            return n;
+        };
+        most = longest;
+        while (most > 1 && records(most) > room) most = (most + 1) / 2;
+        (void)records(most);
+        if (n_chunked > 65535 || most > 65535) return NVLLM_BAD_SIZE;
+    }
+    const size_t ints = spans.size() * 5 + 4;
+    if (ints > staging_ints()) return NVLLM_BAD_SIZE;
     ensure_init();
     if (stream_is_captured()) return NVLLM_CAPTURED;
-    double state_floats = 0;
-    for (const int4& s : spans) state_floats += (s.z > 0 ? 2.0 : 1.0) * a.H * a.dim * (double)a.vdim;
-    a.n_spans = (int)spans.size();
-    a.spans = nullptr;
-    if (a.n_spans <= DELTA_SPANS) {
-        std::copy(spans.begin(), spans.end(), a.here);
-    } else {
-        int* host = pinned_ints(spans.size() * 4);
+    const int4* d_spans = nullptr;
+    const int* d_first = nullptr;
+    if (spans.size() > DELTA_SPANS) {
+        int* host = pinned_ints(ints);
         std::copy(spans.begin(), spans.end(), (int4*)host);
-        int* dev = (int*)ws_get(WS_STEP, spans.size() * 16);
-        launch_copy_ints(dev, host, spans.size() * 4);
-        a.spans = (const int4*)dev;
+        std::copy(first.begin(), first.end(), host + 4 * spans.size());
+        int* dev = (int*)ws_get(WS_STEP, ints * sizeof(int));
+        launch_copy_ints(dev, host, spans.size() * 5);
+        d_spans = (const int4*)dev;
+        d_first = dev + 4 * spans.size();
     }
-    const bool b16 = elem == 2;
+    const double token_bytes = elem * (2.0 * a.Q * a.dim + 2.0 * a.H * a.vdim) + 8.0 * a.H, token_flops = 6.0 * a.H * a.dim * (double)a.vdim;
+    if (n_chunked > 0) {
+        DeltaChunks c{};
+        c.a = a;
+        c.a.n_spans = n_chunked;
+        c.a.spans = d_spans;
+        c.first = d_first;
+        if (!d_spans) {
+            std::copy(spans.begin(), spans.begin() + n_chunked, c.a.here);
+            std::copy(first.begin(), first.begin() + n_chunked, c.first_here);
+        }
+        c.out_four = a.vdim % 4 == 0 && (size_t)a.out % (4 * elem) == 0;
+        size_t n_records = 0;
+        for (int i = 0; i < n_chunked; i++) n_records = std::max(n_records, (size_t)first[i] + std::min(most, cdiv(spans[i].y, CH)));
+        const int per16 = 16 / elem, dim_ld = (a.dim + 7) & ~7;
+        const bool fits = a.dim % 8 == 0 && a.q_ld % per16 == 0 && a.k_ld % per16 == 0 && ((size_t)a.q | (size_t)a.k) % 16 == 0;
+        const size_t rows = fits ? 0 : (size_t)T * a.Q * dim_ld * elem;
+        const size_t row_room = (rows + 255) & ~(size_t)255;
+        char* mem = (char*)ws_get(WS_DELTA, 2 * row_room + n_records * a.H * DELTA_RECORD);
+        if (!fits) {
+            auto pack = [&](const void* src, long ld, char* dst) {
+                if (b16) NVLLM_LAUNCH((k_delta_rows<unsigned short>), dim3(T), dim3(256), 0, (unsigned short*)dst, (const unsigned short*)src, a.Q, a.dim, dim_ld, ld);
+                else NVLLM_LAUNCH((k_delta_rows<float>), dim3(T), dim3(256), 0, (float*)dst, (const float*)src, a.Q, a.dim, dim_ld, ld);
+            };
+            pack(a.q, a.q_ld, mem);
+            pack(a.k, a.k_ld, mem + row_room);
+            c.a.q = mem;
+            c.a.k = mem + row_room;
+            c.a.q_ld = c.a.k_ld = (long)a.Q * dim_ld;
+            c.a.dim = dim_ld;
+            mem += 2 * row_room;
+        }
+        c.mem = mem;
+        // the algorithm's bytes and flops, split over the launches
+        const int rounds = cdiv(longest, most);
+        c.bytes = (states[1] + (double)tokens * token_bytes) / rounds;
+        c.flops = (double)tokens * token_flops / rounds;
+        for (c.from = 0; c.from < longest; c.from += most) {
+            c.most = std::min(most, longest - c.from);
+            if (b16) launch_chunks<true>(c);
+            else launch_chunks<false>(c);
+        }
+    }
+    a.n_spans = (int)spans.size() - n_chunked;
+    if (a.n_spans == 0) return 0;
+    a.spans = d_spans ? d_spans + n_chunked : nullptr;
+    if (!d_spans) std::copy(spans.begin() + n_chunked, spans.end(), a.here);
     const size_t four = 4 * (size_t)elem;
     const bool vec = a.dim % 4 == 0 && a.vdim % 4 == 0 && a.q_ld % 4 == 0 && a.k_ld % 4 == 0 && a.v_ld % 4 == 0 && (size_t)a.q % four == 0 && (size_t)a.k % four == 0 &&
                      (size_t)a.v % four == 0 && (size_t)a.out % four == 0 && (size_t)a.state % 16 == 0;
-    ProfScope ps(PC_DELTA_TOK, state_floats * 4 + (double)T * (elem * (2.0 * a.Q * a.dim + 2.0 * a.H * a.vdim) + 8.0 * a.H), 6.0 * T * a.H * a.dim * (double)a.vdim);
+    ProfScope ps(PC_DELTA_TOK, states[0] + (double)(T - tokens) * token_bytes, (double)(T - tokens) * token_flops);
     if (b16 && vec) launch_step<true, true>(a);
     else if (b16) launch_step<true, false>(a);
     else if (vec) launch_step<false, true>(a);
@@ -245,7 +835,7 @@ extern "C" int nvllm_gated_delta(void* out, const void* q, const void* k, const 
     a.q = q; a.k = k; a.v = v; a.g = g; a.beta = beta; a.state = state; a.out = out;
     a.q_ld = q_ld; a.k_ld = k_ld; a.v_ld = v_ld;
     a.scale = scale; a.eps = norm_eps;
-    a.Q = qk_heads; a.H = heads; a.dim = dim; a.vdim = vdim;
+    a.Q = qk_heads; a.H = heads; a.dim = a.dim_kept = dim; a.vdim = vdim;
     try {
         return gated_delta(a, seq_ids, pos_arr, num_tokens, n_slots, elem_bytes);
     } catch (const std::bad_alloc&) {
