@@ -232,6 +232,15 @@ __device__ __forceinline__ f4_t mfma6(const b8_t (&a)[3], const b8_t (&b)[3], f4
 __device__ __forceinline__ f4_t mfma4(float a, float b, const f4_t& c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ float exp_of(double x) { return __builtin_amdgcn_exp2f((float)(x * 1.4426950408889634)); }
 
+// Memory by descriptors: what lies behind `bytes` (and every offset of NOWHERE) reads as zeros and is not written, so that a chunk's
+// loads have no branch around them and all of them are in flight together.
+constexpr unsigned NOWHERE = 0x80000000u;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t memory(const void* base, long bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)bytes, 0x00020000);
+}
+__device__ __forceinline__ u4_t load16(__amdgpu_buffer_rsrc_t m, unsigned at) { return __builtin_bit_cast(u4_t, __builtin_amdgcn_raw_buffer_load_b128(m, (int)at, 0, 0)); }
+__device__ __forceinline__ float load4(__amdgpu_buffer_rsrc_t m, unsigned at) { return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(m, (int)at, 0, 0)); }
+
 // A token's row of queries or keys as operands: lane (x, g) has dims 32 cc + 8 g .. + 7 of the tile's row x.
 template <int DC, bool B16>
 struct Rows {
@@ -246,6 +255,15 @@ struct Rows {
                 w[cc][i] = u4_t{0, 0, 0, 0};
                 if (there && d < dim) w[cc][i] = *reinterpret_cast<const u4_t*>((const char*)base + (row + d) * (B16 ? 2 : 4) + 16 * i);
             }
+        }
+    }
+    // row: the offset of a token's row in bytes
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t m, unsigned row, int dim, int g) {
+#pragma unroll
+        for (int cc = 0; cc < DC; cc++) {
+            const unsigned d = 32 * cc + 8 * g, at = (int)d < dim ? row + d * (B16 ? 2 : 4) : NOWHERE;
+#pragma unroll
+            for (int i = 0; i < W; i++) w[cc][i] = load16(m, at + 16 * i);
         }
     }
     __device__ __forceinline__ void operand(int cc, b8_t (&p)[B16 ? 1 : 3]) const {
@@ -279,6 +297,12 @@ __device__ __forceinline__ f4_t mfma_rows(const b8_t (&a)[B16 ? 1 : 3], const b8
     else return mfma6(a, b, c);
 }
 
+// a portion of the launch, and its first record, in scalar registers
+__device__ __forceinline__ int4 span_of(const Delta& a, int s) {
+    const int4 v = a.spans ? a.spans[s] : a.here[s];
+    return int4{__builtin_amdgcn_readfirstlane(v.x), __builtin_amdgcn_readfirstlane(v.y), __builtin_amdgcn_readfirstlane(v.z), __builtin_amdgcn_readfirstlane(v.w)};
+}
+__device__ __forceinline__ int first_of(const DeltaChunks& c, int s) { return __builtin_amdgcn_readfirstlane(c.first ? c.first[s] : c.first_here[s]); }
 struct ChunkAt {
     int4 span;
     int first, n;   // token of the batch, tokens
@@ -286,10 +310,10 @@ struct ChunkAt {
 };
 __device__ __forceinline__ ChunkAt chunk_at(const DeltaChunks& c, int s, int h, int i) {
     ChunkAt at;
-    at.span = (c.a.spans ? c.a.spans : c.a.here)[s];
+    at.span = span_of(c.a, s);
     at.first = at.span.x + (c.from + i) * CH;
     at.n = min(CH, at.span.y - (c.from + i) * CH);
-    at.record = c.mem + ((size_t)((c.first ? c.first : c.first_here)[s] + i) * c.a.H + h) * DELTA_RECORD;
+    at.record = c.mem + ((size_t)(first_of(c, s) + i) * c.a.H + h) * DELTA_RECORD;
     return at;
 }
 // T' and P: tile (token tile w, 32 tokens p) of the six that are not empty
@@ -467,7 +491,7 @@ constexpr int chunks_lds() { return (3 * DC + 6 + 6 + 6) * 1024 + (B16 ? 1 : 3) 
 
 template <int DC, bool B16>
 __global__ __launch_bounds__(256) void k_delta_chunks(DeltaChunks c) {
-    constexpr int PARTS = B16 ? 1 : 3, TILES = (2 * DC + 3) / 4, ROW = 32 * DC + 8;
+    constexpr int PARTS = B16 ? 1 : 3, TILES = (2 * DC + 3) / 4, ROW = 32 * DC + 8, ELEM = B16 ? 2 : 4;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds_d[];
     u4_t* s_S = reinterpret_cast<u4_t*>(lds_d);   // [DC][part][64]
     u4_t* s_X = s_S + DC * 3 * 64;                // [32 tokens][part][64]
@@ -477,11 +501,11 @@ __global__ __launch_bounds__(256) void k_delta_chunks(DeltaChunks c) {
     const Delta& a = c.a;
     const int h = blockIdx.x, slice = blockIdx.y, hq = h / (a.H / a.Q);
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), x = lane & 15, g = lane >> 4;
-    const int4 span = (a.spans ? a.spans : a.here)[blockIdx.z];
+    const int4 span = span_of(a, blockIdx.z);
     const int chunks = min(c.most, (span.y + CH - 1) / CH - c.from);
     if (chunks <= 0) return;
     const int col = slice * 16 + x;   // of the state, of V
-    const bool has_col = col < a.vdim, upper = w >= 2;
+    const bool has_col = col < a.vdim;
     float* st = a.state + ((size_t)span.w * a.H + h) * a.dim_kept * a.vdim;
     // ---- the state: this wave's tiles, and all of them as operands
     f4_t S[TILES];
@@ -505,46 +529,52 @@ __global__ __launch_bounds__(256) void k_delta_chunks(DeltaChunks c) {
     auto put_state = [&] {
 #pragma unroll
         for (int j = 0; j < TILES; j++)
-            if (w + 4 * j < 2 * DC) put(s_S + ((w + 4 * j) >> 1) * 3 * 64, w & 1, S[j]);
+            if (2 * DC % 4 == 0 || w + 4 * j < 2 * DC) put(s_S + ((w + 4 * j) >> 1) * 3 * 64, w & 1, S[j]);
     };
     put_state();
     // ---- a chunk's rows, factors and operands, each asked for when the last chunk's are used
+    const int first = span.x + c.from * CH, tokens = min(span.y - c.from * CH, chunks * CH);
+    const char* record = c.mem + ((size_t)first_of(c, blockIdx.z) * a.H + h) * DELTA_RECORD;
+    const unsigned k_row = (16 * w + x) * (unsigned)a.k_ld * ELEM, q_row = (16 * w + x) * (unsigned)a.q_ld * ELEM;
+    const unsigned v_ld = (unsigned)a.v_ld * ELEM, v_row = has_col ? (16 * w + 4 * g) * v_ld + x * ELEM : NOWHERE;
+    const unsigned op0 = op_tile(w, 0) * DELTA_TILE + lane * 16, op1 = w >= 2 ? op0 + DELTA_TILE : NOWHERE;   // (no tokens behind the wave's own)
+    const unsigned o_row = ((16 * w + x) * (unsigned)(a.H * a.vdim) + 4 * g) * ELEM;
+    bool has_out[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) has_out[e] = slice * 16 + 4 * g + e < a.vdim;
     Rows<DC, B16> k, q;
-    float v[4], fb, fade;
+    unsigned v[4];
+    float fb, fade;
     f4_t fa, fc;
     b8_t to[2][3], po[2][3];
+    auto rows_of = [&](const void* base, long ld, int at, int i, int width) {   // of chunk i's tokens
+        const int n = min(CH, tokens - i * CH);
+        return memory((const char*)base + ((size_t)(first + i * CH) * ld + at) * ELEM, ((n - 1) * ld + width) * ELEM);
+    };
+    auto record_of = [&](int i) { return memory(record + (size_t)i * a.H * DELTA_RECORD, DELTA_RECORD); };
     auto fetch_rows = [&](int i) {
-        const ChunkAt at = chunk_at(c, blockIdx.z, h, i);
-        const int t = 16 * w + x;
-        k.load(a.k, (size_t)(at.first + t) * a.k_ld + hq * a.dim, a.dim, g, t < at.n);
-        q.load(a.q, (size_t)(at.first + t) * a.q_ld + hq * a.dim, a.dim, g, t < at.n);
+        k.load(rows_of(a.k, a.k_ld, hq * a.dim, i, a.dim), k_row, a.dim, g);
+        q.load(rows_of(a.q, a.q_ld, hq * a.dim, i, a.dim), q_row, a.dim, g);
+        const auto mv = rows_of(a.v, a.v_ld, h * a.vdim + slice * 16, i, min(16, a.vdim - slice * 16));
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const int tok = 16 * w + 4 * g + r;
-            v[r] = 0.f;
-            if (tok < at.n && has_col) {
-                const size_t e = (size_t)(at.first + tok) * a.v_ld + h * a.vdim + col;
-                v[r] = B16 ? __builtin_bit_cast(float, (unsigned)((const unsigned short*)a.v)[e] << 16) : ((const float*)a.v)[e];
-            }
-        }
-        const float* f = reinterpret_cast<const float*>(at.record + DELTA_OPS);
-        fa = *reinterpret_cast<const f4_t*>(f + 16 * w + 4 * g);
-        fb = f[CH + t];
+        for (int r = 0; r < 4; r++)
+            v[r] = B16 ? (unsigned)__builtin_amdgcn_raw_buffer_load_b16(mv, (int)(v_row + r * v_ld), 0, 0) : __builtin_amdgcn_raw_buffer_load_b32(mv, (int)(v_row + r * v_ld), 0, 0);
+        const auto m = record_of(i);
+        fa = __builtin_bit_cast(f4_t, load16(m, DELTA_OPS + (16 * w + 4 * g) * 4));
+        fb = load4(m, DELTA_OPS + (CH + 16 * w + x) * 4);
     };
     auto fetch_ops = [&](int i, int what, b8_t (&o)[2][3]) {
-        const u4_t* ops = reinterpret_cast<const u4_t*>(chunk_at(c, blockIdx.z, h, i).record) + lane;
+        const auto m = record_of(i);
 #pragma unroll
-        for (int p = 0; p < 2; p++)
-#pragma unroll
-            for (int j = 0; j < 3; j++) {
-                o[p][j] = b8_t{};
-                if (p == 0 || upper) o[p][j] = __builtin_bit_cast(b8_t, ops[((what * 6 + op_tile(w, p)) * 3 + j) * 64]);
-            }
+        for (int j = 0; j < 3; j++) {
+            o[0][j] = __builtin_bit_cast(b8_t, load16(m, op0 + what * 6 * DELTA_TILE + j * DELTA_PART));
+            o[1][j] = __builtin_bit_cast(b8_t, load16(m, op1 + what * 6 * DELTA_TILE + j * DELTA_PART));
+        }
     };
     auto fetch_factors = [&](int i) {
-        const float* f = reinterpret_cast<const float*>(chunk_at(c, blockIdx.z, h, i).record + DELTA_OPS);
-        fc = *reinterpret_cast<const f4_t*>(f + 2 * CH + 16 * w + 4 * g);
-        fade = f[3 * CH];
+        const auto m = record_of(i);
+        fc = __builtin_bit_cast(f4_t, load16(m, DELTA_OPS + (2 * CH + 16 * w + 4 * g) * 4));
+        fade = load4(m, DELTA_OPS + 3 * CH * 4);
     };
     fetch_rows(0);
     fetch_ops(0, 0, to);
@@ -552,7 +582,6 @@ __global__ __launch_bounds__(256) void k_delta_chunks(DeltaChunks c) {
     fetch_ops(0, 1, po);
     __syncthreads();
     for (int i = 0; i < chunks; i++) {
-        const ChunkAt at = chunk_at(c, blockIdx.z, h, i);
         const int next = min(i + 1, chunks - 1);
         // ---- S^T k and S^T q
         f4_t D[2] = {}, O[2] = {};
@@ -578,22 +607,21 @@ __global__ __launch_bounds__(256) void k_delta_chunks(DeltaChunks c) {
         f4_t X;
         const f4_t d = D[0] + D[1];
 #pragma unroll
-        for (int r = 0; r < 4; r++) X[r] = fmaf(-fa[r], d[r], v[r]);
+        for (int r = 0; r < 4; r++) {
+            const unsigned bits = B16 ? v[r] << 16 : v[r];
+            X[r] = fmaf(-fa[r], d[r], __builtin_bit_cast(float, bits));
+        }
         f4_t o = (O[0] + O[1]) * fb;
         put(s_X + (w >> 1) * 3 * 64, w & 1, X);
         fetch_rows(next);
         __syncthreads();
         // ---- U = T' X
-        f4_t U = {0.f, 0.f, 0.f, 0.f};
-        b8_t e[3];
-        get(s_X, e);
-        U = mfma6(to[0], e, U);
-        if (upper) {
-            get(s_X + 3 * 64, e);
-            U = mfma6(to[1], e, U);
-        }
-        put(s_U + (w >> 1) * 3 * 64, w & 1, U);
+        b8_t e[2][3];
+        get(s_X, e[0]);
+        get(s_X + 3 * 64, e[1]);
+        const f4_t U = mfma6(to[0], e[0], f4_t{0.f, 0.f, 0.f, 0.f}) + mfma6(to[1], e[1], f4_t{0.f, 0.f, 0.f, 0.f});
         put(s_V + (w >> 1) * 3 * 64, w & 1, U * fc);
+        put(s_U + (w >> 1) * 3 * 64, w & 1, U);
         const float left = fade;
         fetch_ops(next, 0, to);
         fetch_factors(next);
@@ -602,10 +630,12 @@ __global__ __launch_bounds__(256) void k_delta_chunks(DeltaChunks c) {
         b8_t u[2][3];
         get(s_V, u[0]);
         get(s_V + 3 * 64, u[1]);
+        get(s_U, e[0]);
+        get(s_U + 3 * 64, e[1]);
 #pragma unroll
         for (int j = 0; j < TILES; j++) {
             const int tile = w + 4 * j;
-            if (tile >= 2 * DC) break;
+            if (2 * DC % 4 != 0 && tile >= 2 * DC) break;
             S[j] *= left;
 #pragma unroll
             for (int p = 0; p < 2; p++) {
@@ -625,18 +655,19 @@ __global__ __launch_bounds__(256) void k_delta_chunks(DeltaChunks c) {
         }
         put_state();
         // ---- the results: lane (x, g) has token 16 w + x, columns 4 g .. + 3
-        get(s_U, e);
-        o = mfma6(e, po[0], o);
-        if (upper) {
-            get(s_U + 3 * 64, e);
-            o = mfma6(e, po[1], o);
-        }
+        o = mfma6(e[0], po[0], o) + mfma6(e[1], po[1], f4_t{0.f, 0.f, 0.f, 0.f});
         fetch_ops(next, 1, po);
-        if (16 * w + x < at.n) {
-            const int oc = slice * 16 + 4 * g;
-            const size_t e0 = ((size_t)(at.first + 16 * w + x) * a.H + h) * a.vdim + oc;
-            if (c.out_four) store_four<B16, true>(a.out, e0, o, a.vdim - oc);
-            else store_four<B16, false>(a.out, e0, o, a.vdim - oc);
+        const auto mo = rows_of(a.out, (long)a.H * a.vdim, h * a.vdim + slice * 16, i, min(16, a.vdim - slice * 16));
+        if (c.out_four) {
+            if (B16) __builtin_amdgcn_raw_buffer_store_b64(u2_t{two_b16(o[0], o[1]), two_b16(o[2], o[3])}, mo, (int)(has_out[0] ? o_row : NOWHERE), 0, 0);
+            else __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4_t, o), mo, (int)(has_out[0] ? o_row : NOWHERE), 0, 0);
+        } else {
+#pragma unroll
+            for (int e1 = 0; e1 < 4; e1++) {
+                const float y = o[e1];
+                if (B16) __builtin_amdgcn_raw_buffer_store_b16((unsigned short)two_b16(y, y), mo, (int)(has_out[e1] ? o_row + 2 * e1 : NOWHERE), 0, 0);
+                else __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, y), mo, (int)(has_out[e1] ? o_row + 4 * e1 : NOWHERE), 0, 0);
+            }
         }
         __syncthreads();
     }
@@ -828,6 +859,7 @@ extern "C" int nvllm_gated_delta(void* out, const void* q, const void* k, const 
     if (num_tokens == 0) return 0;
     if (!out || !q || !k || !v || !g || !beta || !state || !seq_ids || !pos_arr || n_slots <= 0 || qk_heads <= 0 || heads <= 0 || dim <= 0 || vdim <= 0 || !(norm_eps >= 0.f))
         return NVLLM_BAD_ARGUMENT;
+    if (std::max(std::max(q_ld, k_ld), v_ld) > 1 << 23 || (long)heads * vdim > 1 << 23) return NVLLM_BAD_SIZE;   // (offsets inside a chunk are 31 bits)
     if ((elem_bytes != 2 && elem_bytes != 4) || dim > DELTA_MAX_DIM || heads % qk_heads || heads > 65535 || vdim > 65535) return NVLLM_BAD_SIZE;
     if (q_ld < (long)qk_heads * dim || k_ld < (long)qk_heads * dim || v_ld < (long)heads * vdim) return NVLLM_BAD_ARGUMENT;
     if (((size_t)q | (size_t)k | (size_t)v | (size_t)out) % elem_bytes || ((size_t)g | (size_t)beta | (size_t)state) % 4) return NVLLM_BAD_ARGUMENT;
