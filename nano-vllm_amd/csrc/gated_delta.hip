@@ -483,85 +483,42 @@ __global__ __launch_bounds__(256) void k_delta_prepare(DeltaChunks c) {
         }
 }
 
-// A workgroup = (portion, head, 16 value columns); wave w has tokens 16 w .. + 15 of a chunk and the state's dim tiles w, w + 4, ..
-// A dim tile's row 4 g + r is dim 32 (i / 2) + 8 g + 4 (i & 1) + r, so that a lane's eight values of two tiles are the k of one
-// operand and a row's 16 bytes of keys are the other.
+// A workgroup = (portion, head, 16 value columns).  Waves 0 .. 3 walk the chain, in which every chunk waits for the last one: wave w
+// keeps the state's 32 dims w (and w + 4) in registers and forms their share of S^T k for all 64 tokens; the shares meet in LDS,
+// and wave w goes on with tokens 16 w .. + 15 up to U, which all of them take for their dims.  Waves 4 .. 7 form the results of 16
+// tokens each beside it, from the state and U as the chain leaves them in LDS.  A state's two tiles of 16 dims have dim 8 g + 4 half + r of
+// the 32 in row 4 g + r, so that a lane's eight values are the k of one operand and 16 bytes of a row of keys are the other.
+// Chunks of 128 x 128 heads, one workgroup per CU: 5,600 clocks with both on the same four waves.
 template <int DC, bool B16>
-constexpr int chunks_lds() { return (3 * DC + 6 + 6 + 6) * 1024 + (B16 ? 1 : 3) * CH * (32 * DC + 8) * 2; }
+constexpr int chunks_lds() { return 3 * DC * 1024 + 16 * 1024 + 18 * 1024 + (B16 ? 1 : 3) * DC * 4096; }
 
 template <int DC, bool B16>
-__global__ __launch_bounds__(256) void k_delta_chunks(DeltaChunks c) {
-    constexpr int PARTS = B16 ? 1 : 3, TILES = (2 * DC + 3) / 4, ROW = 32 * DC + 8, ELEM = B16 ? 2 : 4;
+__global__ __launch_bounds__(512) void k_delta_chunks(DeltaChunks c) {
+    constexpr int PARTS = B16 ? 1 : 3, OWN = (DC + 3) / 4, SHARES = DC < 4 ? DC : 4, ELEM = B16 ? 2 : 4, W = B16 ? 1 : 2;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds_d[];
-    u4_t* s_S = reinterpret_cast<u4_t*>(lds_d);   // [DC][part][64]
-    u4_t* s_X = s_S + DC * 3 * 64;                // [32 tokens][part][64]
+    u4_t* s_S = reinterpret_cast<u4_t*>(lds_d);          // [DC][part][64] the state as operand
+    f4_t* s_D = reinterpret_cast<f4_t*>(s_S + DC * 192);  // [wave][token tile][64] shares of S^T k
+    u4_t* s_X = reinterpret_cast<u4_t*>(s_D + 16 * 64);   // [32 tokens][part][64]
     u4_t* s_U = s_X + 6 * 64;
-    u4_t* s_V = s_U + 6 * 64;                     // U as the state takes it
-    unsigned short* s_k = reinterpret_cast<unsigned short*>(s_V + 6 * 64);   // [part][token][ROW]
+    u4_t* s_V = s_U + 6 * 64;                            // U as the state takes it
+    u4_t* s_k = s_V + 6 * 64;                            // [DC][part][token][4] 32 dims of the keys
     const Delta& a = c.a;
     const int h = blockIdx.x, slice = blockIdx.y, hq = h / (a.H / a.Q);
-    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), x = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3, x = lane & 15, g = lane >> 4;
     const int4 span = span_of(a, blockIdx.z);
     const int chunks = min(c.most, (span.y + CH - 1) / CH - c.from);
     if (chunks <= 0) return;
-    const int col = slice * 16 + x;   // of the state, of V
-    const bool has_col = col < a.vdim;
-    float* st = a.state + ((size_t)span.w * a.H + h) * a.dim_kept * a.vdim;
-    // ---- the state: this wave's tiles, and all of them as operands
-    f4_t S[TILES];
-    auto dim_of = [&](int i) { return 32 * (i >> 1) + 8 * g + 4 * (i & 1); };
-#pragma unroll
-    for (int j = 0; j < TILES; j++) {
-        const int i = w + 4 * j, d0 = dim_of(i);
-#pragma unroll
-        for (int r = 0; r < 4; r++) S[j][r] = span.z + c.from > 0 && has_col && i < 2 * DC && d0 + r < a.dim_kept ? st[(size_t)(d0 + r) * a.vdim + col] : 0.f;
-    }
-    auto put = [&](u4_t* to, int half, const f4_t& v) {   // [part][64] operands: one half of a lane's eight values
-        u2_t parts[3];
-        parts_of_four(v, parts);
-#pragma unroll
-        for (int p = 0; p < 3; p++) reinterpret_cast<u2_t*>(to + p * 64 + lane)[half] = parts[p];
-    };
-    auto get = [&](const u4_t* from, b8_t (&p)[3]) {
-#pragma unroll
-        for (int j = 0; j < 3; j++) p[j] = __builtin_bit_cast(b8_t, from[j * 64 + lane]);
-    };
-    auto put_state = [&] {
-#pragma unroll
-        for (int j = 0; j < TILES; j++)
-            if (2 * DC % 4 == 0 || w + 4 * j < 2 * DC) put(s_S + ((w + 4 * j) >> 1) * 3 * 64, w & 1, S[j]);
-    };
-    put_state();
-    // ---- a chunk's rows, factors and operands, each asked for when the last chunk's are used
     const int first = span.x + c.from * CH, tokens = min(span.y - c.from * CH, chunks * CH);
     const char* record = c.mem + ((size_t)first_of(c, blockIdx.z) * a.H + h) * DELTA_RECORD;
-    const unsigned k_row = (16 * w + x) * (unsigned)a.k_ld * ELEM, q_row = (16 * w + x) * (unsigned)a.q_ld * ELEM;
-    const unsigned v_ld = (unsigned)a.v_ld * ELEM, v_row = has_col ? (16 * w + 4 * g) * v_ld + x * ELEM : NOWHERE;
     const unsigned op0 = op_tile(w, 0) * DELTA_TILE + lane * 16, op1 = w >= 2 ? op0 + DELTA_TILE : NOWHERE;   // (no tokens behind the wave's own)
-    const unsigned o_row = ((16 * w + x) * (unsigned)(a.H * a.vdim) + 4 * g) * ELEM;
-    bool has_out[4];
-#pragma unroll
-    for (int e = 0; e < 4; e++) has_out[e] = slice * 16 + 4 * g + e < a.vdim;
-    Rows<DC, B16> k, q;
-    unsigned v[4];
-    float fb, fade;
-    f4_t fa, fc;
-    b8_t to[2][3], po[2][3];
     auto rows_of = [&](const void* base, long ld, int at, int i, int width) {   // of chunk i's tokens
         const int n = min(CH, tokens - i * CH);
         return memory((const char*)base + ((size_t)(first + i * CH) * ld + at) * ELEM, ((n - 1) * ld + width) * ELEM);
     };
     auto record_of = [&](int i) { return memory(record + (size_t)i * a.H * DELTA_RECORD, DELTA_RECORD); };
-    auto fetch_rows = [&](int i) {
-        k.load(rows_of(a.k, a.k_ld, hq * a.dim, i, a.dim), k_row, a.dim, g);
-        q.load(rows_of(a.q, a.q_ld, hq * a.dim, i, a.dim), q_row, a.dim, g);
-        const auto mv = rows_of(a.v, a.v_ld, h * a.vdim + slice * 16, i, min(16, a.vdim - slice * 16));
+    auto get = [&](const u4_t* from, b8_t (&p)[3]) {
 #pragma unroll
-        for (int r = 0; r < 4; r++)
-            v[r] = B16 ? (unsigned)__builtin_amdgcn_raw_buffer_load_b16(mv, (int)(v_row + r * v_ld), 0, 0) : __builtin_amdgcn_raw_buffer_load_b32(mv, (int)(v_row + r * v_ld), 0, 0);
-        const auto m = record_of(i);
-        fa = __builtin_bit_cast(f4_t, load16(m, DELTA_OPS + (16 * w + 4 * g) * 4));
-        fb = load4(m, DELTA_OPS + (CH + 16 * w + x) * 4);
+        for (int j = 0; j < 3; j++) p[j] = __builtin_bit_cast(b8_t, from[j * 64 + lane]);
     };
     auto fetch_ops = [&](int i, int what, b8_t (&o)[2][3]) {
         const auto m = record_of(i);
@@ -571,112 +528,207 @@ __global__ __launch_bounds__(256) void k_delta_chunks(DeltaChunks c) {
             o[1][j] = __builtin_bit_cast(b8_t, load16(m, op1 + what * 6 * DELTA_TILE + j * DELTA_PART));
         }
     };
-    auto fetch_factors = [&](int i) {
-        const auto m = record_of(i);
-        fc = __builtin_bit_cast(f4_t, load16(m, DELTA_OPS + (2 * CH + 16 * w + 4 * g) * 4));
-        fade = load4(m, DELTA_OPS + 3 * CH * 4);
-    };
-    fetch_rows(0);
-    fetch_ops(0, 0, to);
-    fetch_factors(0);
-    fetch_ops(0, 1, po);
-    __syncthreads();
-    for (int i = 0; i < chunks; i++) {
-        const int next = min(i + 1, chunks - 1);
-        // ---- S^T k and S^T q
-        f4_t D[2] = {}, O[2] = {};
+    const f4_t zero = {0.f, 0.f, 0.f, 0.f};
+    if (wave < 4) {
+        const int col = slice * 16 + x;   // of the state, of V
+        const bool has_col = col < a.vdim;
+        float* st = a.state + ((size_t)span.w * a.H + h) * a.dim_kept * a.vdim;
+        f4_t S[OWN][2];
+        auto state_at = [&](int j, int half) { return 32 * (w + 4 * j) + 8 * g + 4 * half; };
 #pragma unroll
-        for (int cc = 0; cc < DC; cc++) {
-            b8_t s[3], kp[PARTS], qp[PARTS];
-            get(s_S + cc * 3 * 64, s);
-            k.operand(cc, kp);
-            q.operand(cc, qp);
+        for (int j = 0; j < OWN; j++)
 #pragma unroll
-            for (int p = 0; p < PARTS; p++) *reinterpret_cast<u4_t*>(s_k + (p * CH + 16 * w + x) * ROW + 32 * cc + 8 * g) = __builtin_bit_cast(u4_t, kp[p]);
-            if constexpr (B16) {
+            for (int half = 0; half < 2; half++)
 #pragma unroll
-                for (int p = 2; p >= 0; p--) {
-                    D[p & 1] = mfma(kp[0], s[p], D[p & 1]);
-                    O[p & 1] = mfma(s[p], qp[0], O[p & 1]);
+                for (int r = 0; r < 4; r++) {
+                    const int d = state_at(j, half) + r;
+                    S[j][half][r] = span.z + c.from > 0 && has_col && d < a.dim_kept ? st[(size_t)d * a.vdim + col] : 0.f;
                 }
-            } else {
-                D[cc & 1] = mfma6(kp, s, D[cc & 1]);
-                O[cc & 1] = mfma6(s, qp, O[cc & 1]);
+        // a chunk's keys of the wave's dims, values and factors of its tokens, T': each asked for when the last chunk's are used
+        u4_t k[OWN][4][W];
+        unsigned v[4];
+        f4_t fa, fc;
+        float fade;
+        b8_t to[2][3];
+        const unsigned v_ld = (unsigned)a.v_ld * ELEM, v_row = has_col ? (16 * w + 4 * g) * v_ld + x * ELEM : NOWHERE;
+        auto fetch_keys = [&](int i) {
+            const auto m = rows_of(a.k, a.k_ld, hq * a.dim, i, a.dim);
+#pragma unroll
+            for (int j = 0; j < OWN; j++) {
+                const int d = 32 * (w + 4 * j) + 8 * g;
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int e = 0; e < W; e++) k[j][t][e] = load16(m, d < a.dim ? (unsigned)((16 * t + x) * a.k_ld + d) * ELEM + 16 * e : NOWHERE);
+            }
+        };
+        auto fetch_values = [&](int i) {
+            const auto m = rows_of(a.v, a.v_ld, h * a.vdim + slice * 16, i, min(16, a.vdim - slice * 16));
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+                v[r] = B16 ? (unsigned)__builtin_amdgcn_raw_buffer_load_b16(m, (int)(v_row + r * v_ld), 0, 0) : __builtin_amdgcn_raw_buffer_load_b32(m, (int)(v_row + r * v_ld), 0, 0);
+            fa = __builtin_bit_cast(f4_t, load16(record_of(i), DELTA_OPS + (16 * w + 4 * g) * 4));
+        };
+        auto fetch_factors = [&](int i) {
+            const auto m = record_of(i);
+            fc = __builtin_bit_cast(f4_t, load16(m, DELTA_OPS + (2 * CH + 16 * w + 4 * g) * 4));
+            fade = load4(m, DELTA_OPS + 3 * CH * 4);
+        };
+        auto put = [&](u4_t* to, const f4_t& val) {   // [part][64] operands: this tile's half of a lane's eight values
+            u2_t parts[3];
+            parts_of_four(val, parts);
+#pragma unroll
+            for (int p = 0; p < 3; p++) reinterpret_cast<u2_t*>(to + p * 64 + lane)[w & 1] = parts[p];
+        };
+        fetch_keys(0);
+        fetch_values(0);
+        fetch_factors(0);
+        fetch_ops(0, 0, to);
+        for (int i = 0; i < chunks; i++) {
+            const int next = min(i + 1, chunks - 1);
+            // ---- shares of S^T k
+            f4_t D[4] = {zero, zero, zero, zero};
+#pragma unroll
+            for (int j = 0; j < OWN; j++) {
+                const int cc = w + 4 * j;
+                if (DC % 4 != 0 && cc >= DC) break;
+                b8_t s[3];
+                parts_of_eight(S[j][0], S[j][1], s);
+#pragma unroll
+                for (int p = 0; p < 3; p++) s_S[(cc * 3 + p) * 64 + lane] = __builtin_bit_cast(u4_t, s[p]);
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    b8_t kp[PARTS];
+                    if constexpr (B16) kp[0] = __builtin_bit_cast(b8_t, k[j][t][0]);
+                    else parts_of_eight(__builtin_bit_cast(f4_t, k[j][t][0]), __builtin_bit_cast(f4_t, k[j][t][1]), kp);
+#pragma unroll
+                    for (int p = 0; p < PARTS; p++) s_k[((cc * PARTS + p) * CH + 16 * t + x) * 4 + g] = __builtin_bit_cast(u4_t, kp[p]);
+                    if constexpr (B16) {
+#pragma unroll
+                        for (int p = 2; p >= 0; p--) D[t] = mfma(kp[0], s[p], D[t]);
+                    } else D[t] = mfma6(kp, s, D[t]);
+                }
+            }
+            if (SHARES == 4 || w < SHARES)
+#pragma unroll
+                for (int t = 0; t < 4; t++) s_D[(w * 4 + t) * 64 + lane] = D[t];
+            fetch_keys(next);
+            __syncthreads();
+            // ---- X of the wave's tokens
+            f4_t d = s_D[w * 64 + lane];
+#pragma unroll
+            for (int j = 1; j < SHARES; j++) d += s_D[(j * 4 + w) * 64 + lane];
+            f4_t X;
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const unsigned bits = B16 ? v[r] << 16 : v[r];
+                X[r] = fmaf(-fa[r], d[r], __builtin_bit_cast(float, bits));
+            }
+            put(s_X + (w >> 1) * 192, X);
+            fetch_values(next);
+            __syncthreads();
+            // ---- U = T' X
+            b8_t e[2][3];
+            get(s_X, e[0]);
+            get(s_X + 192, e[1]);
+            const f4_t U = mfma6(to[0], e[0], zero) + mfma6(to[1], e[1], zero);
+            put(s_V + (w >> 1) * 192, U * fc);
+            put(s_U + (w >> 1) * 192, U);
+#pragma unroll
+            for (int j = 0; j < OWN; j++) {
+                S[j][0] *= fade;
+                S[j][1] *= fade;
+            }
+            fetch_factors(next);
+            fetch_ops(next, 0, to);
+            __syncthreads();
+            // ---- the state: keys as columns from LDS (16 lanes bring 4 tokens x 16 dims, lane x receives dim x of the four)
+            get(s_V, e[0]);
+            get(s_V + 192, e[1]);
+#pragma unroll
+            for (int j = 0; j < OWN; j++) {
+                const int cc = w + 4 * j;
+                if (DC % 4 != 0 && cc >= DC) break;
+#pragma unroll
+                for (int half = 0; half < 2; half++) {
+#pragma unroll
+                    for (int p = 0; p < 2; p++) {
+                        b8_t kt[PARTS];
+#pragma unroll
+                        for (int part = 0; part < PARTS; part++) {
+                            const u2_t* at = reinterpret_cast<const u2_t*>(s_k + ((cc * PARTS + part) * CH + 32 * p + 4 * g + (x >> 2)) * 4 + (x & 3)) + half;
+                            const u2_t lo = __builtin_bit_cast(u2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)at));
+                            const u2_t hi = __builtin_bit_cast(u2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at + 16 * 8)));
+                            kt[part] = __builtin_bit_cast(b8_t, u4_t{lo[0], lo[1], hi[0], hi[1]});
+                        }
+                        if constexpr (B16) {
+#pragma unroll
+                            for (int part = 2; part >= 0; part--) S[j][half] = mfma(kt[0], e[p][part], S[j][half]);
+                        } else S[j][half] = mfma6(kt, e[p], S[j][half]);
+                    }
+                }
             }
         }
-        f4_t X;
-        const f4_t d = D[0] + D[1];
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const unsigned bits = B16 ? v[r] << 16 : v[r];
-            X[r] = fmaf(-fa[r], d[r], __builtin_bit_cast(float, bits));
-        }
-        f4_t o = (O[0] + O[1]) * fb;
-        put(s_X + (w >> 1) * 3 * 64, w & 1, X);
-        fetch_rows(next);
-        __syncthreads();
-        // ---- U = T' X
-        b8_t e[2][3];
-        get(s_X, e[0]);
-        get(s_X + 3 * 64, e[1]);
-        const f4_t U = mfma6(to[0], e[0], f4_t{0.f, 0.f, 0.f, 0.f}) + mfma6(to[1], e[1], f4_t{0.f, 0.f, 0.f, 0.f});
-        put(s_V + (w >> 1) * 3 * 64, w & 1, U * fc);
-        put(s_U + (w >> 1) * 3 * 64, w & 1, U);
-        const float left = fade;
-        fetch_ops(next, 0, to);
-        fetch_factors(next);
-        __syncthreads();
-        // ---- the state: keys as columns from LDS (16 lanes bring 4 tokens x 16 dims, lane x receives dim x of the four)
-        b8_t u[2][3];
-        get(s_V, u[0]);
-        get(s_V + 3 * 64, u[1]);
-        get(s_U, e[0]);
-        get(s_U + 3 * 64, e[1]);
+        for (int j = 0; j < OWN; j++)
 #pragma unroll
-        for (int j = 0; j < TILES; j++) {
-            const int tile = w + 4 * j;
-            if (2 * DC % 4 != 0 && tile >= 2 * DC) break;
-            S[j] *= left;
+            for (int half = 0; half < 2; half++)
 #pragma unroll
-            for (int p = 0; p < 2; p++) {
-                b8_t kt[PARTS];
-#pragma unroll
-                for (int part = 0; part < PARTS; part++) {
-                    const unsigned short* at_k = s_k + (part * CH + 32 * p + 4 * g + (x >> 2)) * ROW + 32 * (tile >> 1) + 8 * (x & 3) + 4 * (tile & 1);
-                    const u2_t lo = __builtin_bit_cast(u2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)at_k));
-                    const u2_t hi = __builtin_bit_cast(u2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at_k + 16 * ROW)));
-                    kt[part] = __builtin_bit_cast(b8_t, u4_t{lo[0], lo[1], hi[0], hi[1]});
+                for (int r = 0; r < 4; r++) {
+                    const int d = state_at(j, half) + r;
+                    if (has_col && d < a.dim_kept) st[(size_t)d * a.vdim + col] = S[j][half][r];
                 }
+    } else {
+        // ---- results: lane (x, g) has token 16 w + x, columns 4 g .. + 3
+        const unsigned q_row = (16 * w + x) * (unsigned)a.q_ld * ELEM, o_row = ((16 * w + x) * (unsigned)(a.H * a.vdim) + 4 * g) * ELEM;
+        bool has_out[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) has_out[e] = slice * 16 + 4 * g + e < a.vdim;
+        Rows<DC, B16> q;
+        float fb;
+        b8_t po[2][3];
+        auto fetch_queries = [&](int i) {
+            fb = load4(record_of(i), DELTA_OPS + (CH + 16 * w + x) * 4);
+            q.load(rows_of(a.q, a.q_ld, hq * a.dim, i, a.dim), q_row, a.dim, g);
+        };
+        fetch_queries(0);
+        fetch_ops(0, 1, po);
+        for (int i = 0; i < chunks; i++) {
+            const int next = min(i + 1, chunks - 1);
+            __syncthreads();   // the state is there
+            f4_t O[2] = {zero, zero};
+#pragma unroll
+            for (int cc = 0; cc < DC; cc++) {
+                b8_t s[3], qp[PARTS];
+                get(s_S + cc * 192, s);
+                q.operand(cc, qp);
                 if constexpr (B16) {
 #pragma unroll
-                    for (int part = 2; part >= 0; part--) S[j] = mfma(kt[0], u[p][part], S[j]);
-                } else S[j] = mfma6(kt, u[p], S[j]);
+                    for (int p = 2; p >= 0; p--) O[p & 1] = mfma(s[p], qp[0], O[p & 1]);
+                } else O[cc & 1] = mfma6(s, qp, O[cc & 1]);
+            }
+            f4_t o = (O[0] + O[1]) * fb;
+            fetch_queries(next);
+            __syncthreads();
+            __syncthreads();   // U is there
+            b8_t e[2][3];
+            get(s_U, e[0]);
+            get(s_U + 192, e[1]);
+            o = mfma6(e[0], po[0], o) + mfma6(e[1], po[1], zero);
+            fetch_ops(next, 1, po);
+            const auto m = rows_of(a.out, (long)a.H * a.vdim, h * a.vdim + slice * 16, i, min(16, a.vdim - slice * 16));
+            if (c.out_four) {
+                if (B16) __builtin_amdgcn_raw_buffer_store_b64(u2_t{two_b16(o[0], o[1]), two_b16(o[2], o[3])}, m, (int)(has_out[0] ? o_row : NOWHERE), 0, 0);
+                else __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4_t, o), m, (int)(has_out[0] ? o_row : NOWHERE), 0, 0);
+            } else {
+#pragma unroll
+                for (int e1 = 0; e1 < 4; e1++) {
+                    const float y = o[e1];
+                    if (B16) __builtin_amdgcn_raw_buffer_store_b16((unsigned short)two_b16(y, y), m, (int)(has_out[e1] ? o_row + 2 * e1 : NOWHERE), 0, 0);
+                    else __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, y), m, (int)(has_out[e1] ? o_row + 4 * e1 : NOWHERE), 0, 0);
+                }
             }
         }
-        put_state();
-        // ---- the results: lane (x, g) has token 16 w + x, columns 4 g .. + 3
-        o = mfma6(e[0], po[0], o) + mfma6(e[1], po[1], f4_t{0.f, 0.f, 0.f, 0.f});
-        fetch_ops(next, 1, po);
-        const auto mo = rows_of(a.out, (long)a.H * a.vdim, h * a.vdim + slice * 16, i, min(16, a.vdim - slice * 16));
-        if (c.out_four) {
-            if (B16) __builtin_amdgcn_raw_buffer_store_b64(u2_t{two_b16(o[0], o[1]), two_b16(o[2], o[3])}, mo, (int)(has_out[0] ? o_row : NOWHERE), 0, 0);
-            else __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4_t, o), mo, (int)(has_out[0] ? o_row : NOWHERE), 0, 0);
-        } else {
-#pragma unroll
-            for (int e1 = 0; e1 < 4; e1++) {
-                const float y = o[e1];
-                if (B16) __builtin_amdgcn_raw_buffer_store_b16((unsigned short)two_b16(y, y), mo, (int)(has_out[e1] ? o_row + 2 * e1 : NOWHERE), 0, 0);
-                else __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, y), mo, (int)(has_out[e1] ? o_row + 4 * e1 : NOWHERE), 0, 0);
-            }
-        }
-        __syncthreads();
-    }
-#pragma unroll
-    for (int j = 0; j < TILES; j++) {
-        const int i = w + 4 * j, d0 = dim_of(i);
-#pragma unroll
-        for (int r = 0; r < 4; r++)
-            if (has_col && i < 2 * DC && d0 + r < a.dim_kept) st[(size_t)(d0 + r) * a.vdim + col] = S[j][r];
     }
 }
 
@@ -705,7 +757,7 @@ static void launch_chunks_of(const DeltaChunks& c) {
         NVLLM_LAUNCH((k_delta_prepare<DC, B16>), dim3(a.H, c.most, a.n_spans), dim3(256), prep, c);
     }
     ProfScope ps(PC_DELTA, c.bytes / 2, c.flops / 2);
-    NVLLM_LAUNCH((k_delta_chunks<DC, B16>), dim3(a.H, cdiv(a.vdim, 16), a.n_spans), dim3(256), walk, c);
+    NVLLM_LAUNCH((k_delta_chunks<DC, B16>), dim3(a.H, cdiv(a.vdim, 16), a.n_spans), dim3(512), walk, c);
 }
 template <bool B16>
 static void launch_chunks(const DeltaChunks& c) {
