@@ -6,7 +6,7 @@
 
 namespace nvllm {
 
-constexpr int DELTA_SPANS = 32;   // portions that travel with a launch's arguments
+constexpr int DELTA_SPANS = 96;   // portions that travel with a launch's arguments
 constexpr int DELTA_MAX_DIM = 256;
 
 struct Delta {

@@ -73,29 +73,35 @@ __global__ __launch_bounds__(256) void k_copy_slots(CopyArgs a) {
     }
 }
 
-struct Move {
-    int from, to;
+// The moves of a copy as programs: [n + 1] first moves, and the moves (from, to).
+struct CopyPlan {
+    std::vector<int> first, moves;
+    int programs() const { return (int)first.size() - 1; }
+    void add(int from, int to) {
+        moves.push_back(from);
+        moves.push_back(to);
+    }
+    void end() { first.push_back((int)moves.size() / 2); }
 };
-// The moves of a copy as programs: slots that meet are in one, a slot is written after its last reading.  0 or a refusal.
-static int plan_moves(const int* from, const int* to, int n, int n_slots, std::vector<std::vector<Move>>& programs) {
+// Slots that meet are in one program, a slot is written after its last reading.  0 or a refusal.
+static int plan_moves(const int* from, const int* to, int n, int n_slots, CopyPlan& plan) {
+    // slots by number, or by their place among those that occur if they are few of many
     std::vector<int> slots;
-    slots.reserve(2 * (size_t)n);
+    const bool dense = n_slots <= 16384 || n_slots / 8 <= n;
     for (int i = 0; i < n; i++) {
         if (from[i] < 0 || from[i] >= n_slots || to[i] < 0 || to[i] >= n_slots) return NVLLM_BAD_INDEX;
+        if (dense) continue;
         slots.push_back(from[i]);
         slots.push_back(to[i]);
     }
     std::sort(slots.begin(), slots.end());
     slots.erase(std::unique(slots.begin(), slots.end()), slots.end());
-    auto at = [&](int s) { return (int)(std::lower_bound(slots.begin(), slots.end(), s) - slots.begin()); };
-    const int k = (int)slots.size();
-    std::vector<int> source(k, -1), uses(k, 0), group(k);
-    std::vector<char> written(k, 0);
-    std::iota(group.begin(), group.end(), 0);
-    auto root = [&](int x) {
-        while (group[x] != x) x = group[x] = group[group[x]];
-        return x;
-    };
+    auto at = [&](int s) { return dense ? s : (int)(std::lower_bound(slots.begin(), slots.end(), s) - slots.begin()); };
+    auto slot = [&](int k) { return dense ? k : slots[k]; };
+    const int k = dense ? n_slots : (int)slots.size();
+    std::vector<int> source((size_t)k, -1), uses((size_t)k, 0);
+    std::vector<char> written((size_t)k, 0);
+    int count = 0;
     for (int i = 0; i < n; i++) {
         const int d = at(to[i]), s = at(from[i]);
         if (written[d]) return NVLLM_BAD_INDEX;   // two values for one slot
@@ -103,49 +109,87 @@ static int plan_moves(const int* from, const int* to, int n, int n_slots, std::v
         if (s == d) continue;
         source[d] = s;
         uses[s]++;
-        group[root(d)] = root(s);
+        count++;
     }
-    std::vector<Move> order;
-    std::vector<int> ready;
-    for (int d = 0; d < k; d++)
-        if (source[d] >= 0 && uses[d] == 0) ready.push_back(d);
+    plan.first.reserve((size_t)count + 1);
+    plan.moves.reserve(2 * (size_t)count + 8);
+    plan.first.push_back(0);
+    bool apart = true;   // nobody reads what somebody writes
+    for (int i = 0; i < n && apart; i++) apart = source[at(to[i])] < 0 || uses[at(to[i])] == 0;
+    if (apart) {
+        // a fan out of one source falls into programs of a few moves each
+        std::vector<int> by_source((size_t)n), place((size_t)k, -1);
+        int next = 0;
+        for (int i = 0; i < n; i++) {
+            const int d = at(to[i]), s = source[d];
+            if (s < 0) continue;
+            if (place[s] < 0) {
+                place[s] = next;
+                next += uses[s];
+            }
+            by_source[place[s]++] = d;
+        }
+        for (int i = 0, run = 0; i < next; i++) {
+            plan.add(slot(source[by_source[i]]), slot(by_source[i]));
+            run++;
+            if (run == COPY_FAN || i + 1 == next || source[by_source[i + 1]] != source[by_source[i]]) {
+                plan.end();
+                run = 0;
+            }
+        }
+        return 0;
+    }
+    std::vector<int> group((size_t)k), order, ready;   // order: pairs of places, -1: aside
+    std::iota(group.begin(), group.end(), 0);
+    auto root = [&](int x) {
+        while (group[x] != x) x = group[x] = group[group[x]];
+        return x;
+    };
+    for (int i = 0; i < n; i++) {
+        const int d = at(to[i]);
+        if (source[d] < 0) continue;
+        group[root(d)] = root(source[d]);
+        if (uses[d] == 0) ready.push_back(d);
+    }
     while (!ready.empty()) {
         const int d = ready.back(), s = source[d];
         ready.pop_back();
-        order.push_back({s, d});
+        order.insert(order.end(), {s, d});
         source[d] = -1;
         if (--uses[s] == 0 && source[s] >= 0) ready.push_back(s);
     }
-    for (int c = 0; c < k; c++) {
+    for (int i = 0; i < n; i++) {   // what is left are cycles
+        const int c = at(to[i]);
         if (source[c] < 0) continue;
         int d = c;
-        order.push_back({c, -1});
+        order.insert(order.end(), {c, -1});
         while (source[d] != c) {
-            order.push_back({source[d], d});
+            order.insert(order.end(), {source[d], d});
             const int next = source[d];
             source[d] = -1;
             d = next;
         }
-        order.push_back({-1, d});
+        order.insert(order.end(), {-1, d});
         source[d] = -1;
     }
-    // by group; a fan out of one source whose slot stays as it is falls into programs of a few moves each
-    std::vector<int> program_of(k, -1);
-    for (const Move& m : order) {
-        const int r = root(m.to >= 0 ? m.to : m.from);
-        if (program_of[r] < 0) {
-            program_of[r] = (int)programs.size();
-            programs.emplace_back();
-        }
-        programs[program_of[r]].push_back({m.from < 0 ? -1 : slots[m.from], m.to < 0 ? -1 : slots[m.to]});
+    auto group_of = [&](size_t m) { return root(order[m + 1] >= 0 ? order[m + 1] : order[m]); };
+    std::vector<int> size((size_t)k, 0), roots;
+    for (size_t m = 0; m < order.size(); m += 2) {
+        const int r = group_of(m);
+        if (size[r]++ == 0) roots.push_back(r);
     }
-    const size_t whole = programs.size();
-    for (size_t p = 0; p < whole; p++) {
-        const std::vector<Move> moves = programs[p];
-        if ((int)moves.size() <= COPY_FAN || std::any_of(moves.begin(), moves.end(), [&](const Move& m) { return m.from != moves[0].from || m.to < 0; })) continue;
-        programs[p].resize(COPY_FAN);
-        for (size_t i = COPY_FAN; i < moves.size(); i += COPY_FAN)
-            programs.emplace_back(moves.begin() + (long)i, moves.begin() + (long)std::min(moves.size(), i + COPY_FAN));
+    int next = 0;
+    for (int r : roots) {
+        const int had = size[r];
+        size[r] = next;
+        next += had;
+        plan.first.push_back(next);
+    }
+    plan.moves.resize(order.size());
+    for (size_t m = 0; m < order.size(); m += 2) {
+        const size_t place = 2 * (size_t)size[group_of(m)]++;
+        plan.moves[place] = order[m] < 0 ? -1 : slot(order[m]);
+        plan.moves[place + 1] = order[m + 1] < 0 ? -1 : slot(order[m + 1]);
     }
     return 0;
 }
@@ -158,16 +202,10 @@ static void launch_copy(const CopyArgs& a, unsigned most_units, int arrays) {
 }
 
 int copy_slots(const std::vector<SlotArrays>& arrays, int n_slots, const int* from, const int* to, int n) {
-    std::vector<std::vector<Move>> programs;
-    if (const int e = plan_moves(from, to, n, n_slots, programs)) return e;
-    if (programs.empty()) return 0;
-    std::vector<int> ints(programs.size() + 1, 0);
-    for (size_t p = 0; p < programs.size(); p++) ints[p + 1] = ints[p] + (int)programs[p].size();
-    for (const auto& p : programs)
-        for (const Move& m : p) {
-            ints.push_back(m.from);
-            ints.push_back(m.to);
-        }
+    CopyPlan plan;
+    if (const int e = plan_moves(from, to, n, n_slots, plan)) return e;
+    if (plan.moves.empty()) return 0;
+    const size_t ints = plan.first.size() + plan.moves.size();
     size_t bits = 0;   // of every address and size
     for (const SlotArrays& s : arrays) {
         bits |= (size_t)s.base | s.slot_bytes | (s.count > 1 ? s.stride : 0);
@@ -175,19 +213,19 @@ int copy_slots(const std::vector<SlotArrays>& arrays, int n_slots, const int* fr
     }
     const size_t unit = bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 1;
     for (const SlotArrays& s : arrays)
-        if (s.slot_bytes / unit > 0x7fffffff || (double)(s.slot_bytes / unit / 512 + 1) * (double)programs.size() > 2e9) return NVLLM_BAD_SIZE;
-    if (ints.size() > staging_ints()) return NVLLM_BAD_SIZE;
+        if (s.slot_bytes / unit > 0x7fffffff || (double)(s.slot_bytes / unit / 512 + 1) * (double)plan.programs() > 2e9) return NVLLM_BAD_SIZE;
+    if (ints + 4 > staging_ints()) return NVLLM_BAD_SIZE;
     ensure_init();
     if (stream_is_captured()) return NVLLM_CAPTURED;
     CopyArgs a{};
-    a.n_programs = (int)programs.size();
-    if (ints.size() <= COPY_INLINE) {
-        std::copy(ints.begin(), ints.end(), a.here);
-    } else {
-        int* host = pinned_ints((ints.size() + 3) & ~(size_t)3);
-        std::copy(ints.begin(), ints.end(), host);
-        int* dev = (int*)ws_get(WS_STEP, (ints.size() + 4) * sizeof(int));
-        launch_copy_ints(dev, host, ints.size());
+    a.n_programs = plan.programs();
+    const bool here = ints <= COPY_INLINE;
+    int* host = here ? a.here : pinned_ints((ints + 3) & ~(size_t)3);
+    std::copy(plan.first.begin(), plan.first.end(), host);
+    std::copy(plan.moves.begin(), plan.moves.end(), host + plan.first.size());
+    if (!here) {
+        int* dev = (int*)ws_get(WS_STEP, (ints + 4) * sizeof(int));
+        launch_copy_ints(dev, host, ints);
         a.programs = dev;
     }
     for (size_t i = 0; i < arrays.size();) {
@@ -218,17 +256,32 @@ static std::unordered_map<const void*, std::vector<int>>& shared() {
     static std::unordered_map<const void*, std::vector<int>> m;
     return m;
 }
+static unsigned g_changes = 0;   // of the pools that have an entry
+static std::vector<int>* users_of(const KVCacheManager* mgr) {   // null: no forks
+    static const void* pool = nullptr;   // the last one asked for: a table's blocks are freed one by one
+    static std::vector<int>* users = nullptr;
+    static unsigned seen = 0;
+    if (pool != mgr->pool_k || seen != g_changes) {
+        const auto it = shared().find(mgr->pool_k);
+        pool = mgr->pool_k;
+        users = it == shared().end() ? nullptr : &it->second;
+        seen = g_changes;
+    }
+    return users;
+}
 static int more_users(const KVCacheManager* mgr, int block) {
-    if (shared().empty()) return 0;
-    const auto it = shared().find(mgr->pool_k);
-    return it == shared().end() || block < 0 || block >= (int)it->second.size() ? 0 : it->second[block];
+    const std::vector<int>* u = users_of(mgr);
+    return !u || block < 0 || block >= (int)u->size() ? 0 : (*u)[block];
 }
 bool drop_shared_block(const KVCacheManager* mgr, int block) {
     if (more_users(mgr, block) == 0) return false;
-    shared()[mgr->pool_k][block]--;
+    (*users_of(mgr))[block]--;
     return true;
 }
-void forget_shared_blocks(const void* pool_k) { shared().erase(pool_k); }
+void forget_shared_blocks(const void* pool_k) {
+    shared().erase(pool_k);
+    g_changes++;
+}
 
 // which blocks lie on the free stack; empty: the stack is not one of this pool
 static std::vector<char> free_blocks(const KVCacheManager* mgr) {
@@ -302,7 +355,11 @@ int nvllm_fork_tables(KVCacheManager* mgr, const BlockTable* from, int positions
         }
         std::vector<int>* users = nullptr;
         if (whole > 0) {
-            users = &shared()[mgr->pool_k];
+            users = users_of(mgr);
+            if (!users) {
+                users = &shared()[mgr->pool_k];
+                g_changes++;
+            }
             if ((int)users->size() < mgr->num_blocks) users->resize((size_t)mgr->num_blocks, 0);
         }
         if (tail)
@@ -366,11 +423,11 @@ int nvllm_compact_blocks(KVCacheManager* mgr, BlockTable** tables, int n) {
         if (!from.empty())
             if (const int e = copy_slots(arrays, mgr->num_blocks, from.data(), to.data(), (int)from.size())) return e;
         // (nothing below fails)
-        const auto users = shared().find(mgr->pool_k);
+        std::vector<int>* users = users_of(mgr);
         for (size_t i = 0; i < from.size(); i++) {
             is_free[from[i]] = 1;
             is_free[to[i]] = 0;
-            if (users != shared().end()) std::swap(users->second[from[i]], users->second[to[i]]);
+            if (users) std::swap((*users)[from[i]], (*users)[to[i]]);
         }
         for (BlockTable* t : all)
             for (int i = 0; i < t->num_blocks; i++) t->block_indices[i] = place[t->block_indices[i]];
