@@ -18,6 +18,7 @@ struct Delta {
     float scale, eps;           // eps 0: queries and keys as they are
     int Q, H, dim, vdim;
     int dim_kept;               // of the state: dim without padding
+    int v_cols;                 // of v's rows: vdim with padding
     const int4* spans;          // (first token, count, first position, slot); null: the ones here
     int n_spans;
     int4 here[DELTA_SPANS];

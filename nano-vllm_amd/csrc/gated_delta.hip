@@ -199,18 +199,20 @@ __device__ __forceinline__ unsigned two_b16(float lo, float hi) {
     typedef __bf16 b2_t __attribute__((ext_vector_type(2)));
     return __builtin_bit_cast(unsigned, b2_t{(__bf16)lo, (__bf16)hi});
 }
-__device__ __forceinline__ void parts_of_four(const f4_t& v, u2_t (&out)[3]) {
+__device__ __forceinline__ u2_t next_part(f4_t& v) {   // the part of four values, and what it leaves of them
+    u2_t p = {two_b16(v[0], v[1]), two_b16(v[2], v[3])};
+    asm("" : "+v"(p));   // (the upper halves come from these registers, not from roundings of their own)
 #pragma unroll
     for (int i = 0; i < 2; i++) {
-        float lo = v[2 * i], hi = v[2 * i + 1];
-#pragma unroll
-        for (int k = 0; k < 3; k++) {
-            const unsigned p = two_b16(lo, hi);
-            out[k][i] = p;
-            lo -= __builtin_bit_cast(float, p << 16);
-            hi -= __builtin_bit_cast(float, p & 0xffff0000u);
-        }
+        const unsigned two = p[i];
+        v[2 * i] -= __builtin_bit_cast(float, two << 16);
+        v[2 * i + 1] -= __builtin_bit_cast(float, two & 0xffff0000u);
     }
+    return p;
+}
+__device__ __forceinline__ void parts_of_four(f4_t v, u2_t (&out)[3]) {
+#pragma unroll
+    for (int k = 0; k < 3; k++) out[k] = next_part(v);
 }
 __device__ __forceinline__ void parts_of_eight(const f4_t& lo, const f4_t& hi, b8_t (&out)[3]) {
     u2_t l[3], h[3];
@@ -483,54 +485,61 @@ __global__ __launch_bounds__(256) void k_delta_prepare(DeltaChunks c) {
         }
 }
 
-// A workgroup = (portion, head, 16 value columns).  Waves 0 .. 3 walk the chain, in which every chunk waits for the last one: wave w
-// keeps the state's 32 dims w (and w + 4) in registers and forms their share of S^T k for all 64 tokens; the shares meet in LDS,
-// and wave w goes on with tokens 16 w .. + 15 up to U, which all of them take for their dims.  Waves 4 .. 7 form the results of 16
-// tokens each beside it, from the state and U as the chain leaves them in LDS.  A state's two tiles of 16 dims have dim 8 g + 4 half + r of
-// the 32 in row 4 g + r, so that a lane's eight values are the k of one operand and 16 bytes of a row of keys are the other.
-// Chunks of 128 x 128 heads, one workgroup per CU: 5,600 clocks with both on the same four waves.
+// A workgroup = (portion, head, 16 value columns), eight waves.
+//   0 .. 3, the chain, in which every chunk waits for the last one: wave w keeps the state's 32 dims w (and w + 4) in registers and
+//     forms their share of S^T k for all 64 tokens; the shares meet in LDS, wave w goes on with tokens 16 w .. + 15 up to U, which all
+//     of them take for their dims.  A state's two tiles of 16 dims have dim 8 g + 4 half + r of the 32 in row 4 g + r, so that a lane's
+//     eight values are the k of one operand and 16 bytes of a row of keys are the other.
+//   4, 5, the results of 32 tokens each, from the state and U as the chain leaves them in LDS.
+//   6, 7 bring keys, values, T' and factors of coming chunks from memory, one or two chunks ahead, and lay them out in LDS: the chain
+//     itself asks memory for nothing.
+// Three barriers a chunk (a fourth where LDS holds one chunk's keys only).
 template <int DC, bool B16>
-constexpr int chunks_lds() { return 3 * DC * 1024 + 16 * 1024 + 18 * 1024 + (B16 ? 1 : 3) * DC * 4096; }
+struct Walk {
+    static constexpr int PARTS = B16 ? 1 : 3;
+    static constexpr int STATE = DC * DELTA_TILE, SHARES = 16 * 1024, EX = 2 * DELTA_TILE, KEYS = DC * PARTS * 4096, OPS = 7 * DELTA_TILE, VALUES = 4096, FACTORS = 1024;
+    static constexpr int REST = STATE + SHARES + 3 * EX + VALUES + FACTORS, MOST = 160 * 1024;
+    static constexpr bool STAGED = REST + KEYS + OPS <= MOST;                          // T' goes through LDS
+    static constexpr int BUFFERS = REST + EX + 2 * KEYS + OPS <= MOST ? 2 : 1;         // of keys and of U
+    static constexpr int LDS = REST + (BUFFERS - 1) * EX + BUFFERS * KEYS + (STAGED ? OPS : 0);
+};
 
 template <int DC, bool B16>
 __global__ __launch_bounds__(512) void k_delta_chunks(DeltaChunks c) {
-    constexpr int PARTS = B16 ? 1 : 3, OWN = (DC + 3) / 4, SHARES = DC < 4 ? DC : 4, ELEM = B16 ? 2 : 4, W = B16 ? 1 : 2;
+    typedef Walk<DC, B16> L;
+    constexpr int PARTS = L::PARTS, OWN = (DC + 3) / 4, SHARES = DC < 4 ? DC : 4, ELEM = B16 ? 2 : 4;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds_d[];
-    u4_t* s_S = reinterpret_cast<u4_t*>(lds_d);          // [DC][part][64] the state as operand
-    f4_t* s_D = reinterpret_cast<f4_t*>(s_S + DC * 192);  // [wave][token tile][64] shares of S^T k
-    u4_t* s_X = reinterpret_cast<u4_t*>(s_D + 16 * 64);   // [32 tokens][part][64]
-    u4_t* s_U = s_X + 6 * 64;
-    u4_t* s_V = s_U + 6 * 64;                            // U as the state takes it
-    u4_t* s_k = s_V + 6 * 64;                            // [DC][part][token][4] 32 dims of the keys
+    u4_t* s_S = reinterpret_cast<u4_t*>(lds_d);            // [DC][part][64] the state as operand
+    f4_t* s_D = reinterpret_cast<f4_t*>(s_S + DC * 192);   // [wave][token tile][64] shares of S^T k
+    u4_t* s_X = reinterpret_cast<u4_t*>(s_D + 16 * 64);    // [32 tokens][part][64]
+    u4_t* s_U = s_X + 6 * 64;                              // [buffer]
+    u4_t* s_V = s_U + L::BUFFERS * 6 * 64;                 // U as the state takes it
+    u4_t* s_v = s_V + 6 * 64;                              // [token][16] values
+    float* s_f = reinterpret_cast<float*>(s_v + 4 * 64);   // factors a, c, what is left of the state
+    u4_t* s_k = reinterpret_cast<u4_t*>(s_f + 256);        // [buffer][DC][part][token][4] keys, 32 dims together
+    u4_t* s_t = s_k + L::BUFFERS * DC * PARTS * 256;       // T', and a tile of zeros
     const Delta& a = c.a;
     const int h = blockIdx.x, slice = blockIdx.y, hq = h / (a.H / a.Q);
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3, x = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), x = lane & 15, g = lane >> 4;
     const int4 span = span_of(a, blockIdx.z);
     const int chunks = min(c.most, (span.y + CH - 1) / CH - c.from);
     if (chunks <= 0) return;
     const int first = span.x + c.from * CH, tokens = min(span.y - c.from * CH, chunks * CH);
     const char* record = c.mem + ((size_t)first_of(c, blockIdx.z) * a.H + h) * DELTA_RECORD;
-    const unsigned op0 = op_tile(w, 0) * DELTA_TILE + lane * 16, op1 = w >= 2 ? op0 + DELTA_TILE : NOWHERE;   // (no tokens behind the wave's own)
-    auto rows_of = [&](const void* base, long ld, int at, int i, int width) {   // of chunk i's tokens
-        const int n = min(CH, tokens - i * CH);
-        return memory((const char*)base + ((size_t)(first + i * CH) * ld + at) * ELEM, ((n - 1) * ld + width) * ELEM);
+    auto rows_of = [&](const void* base, long ld, int at, int i, int width) {   // of chunk i's tokens; behind the last chunk: the last one's
+        const int ci = min(i, chunks - 1), n = min(CH, tokens - ci * CH);
+        return memory((const char*)base + ((size_t)(first + ci * CH) * ld + at) * ELEM, ((n - 1) * ld + width) * ELEM);
     };
-    auto record_of = [&](int i) { return memory(record + (size_t)i * a.H * DELTA_RECORD, DELTA_RECORD); };
+    auto record_of = [&](int i) { return memory(record + (size_t)min(i, chunks - 1) * a.H * DELTA_RECORD, DELTA_RECORD); };
     auto get = [&](const u4_t* from, b8_t (&p)[3]) {
 #pragma unroll
         for (int j = 0; j < 3; j++) p[j] = __builtin_bit_cast(b8_t, from[j * 64 + lane]);
     };
-    auto fetch_ops = [&](int i, int what, b8_t (&o)[2][3]) {
-        const auto m = record_of(i);
-#pragma unroll
-        for (int j = 0; j < 3; j++) {
-            o[0][j] = __builtin_bit_cast(b8_t, load16(m, op0 + what * 6 * DELTA_TILE + j * DELTA_PART));
-            o[1][j] = __builtin_bit_cast(b8_t, load16(m, op1 + what * 6 * DELTA_TILE + j * DELTA_PART));
-        }
-    };
     const f4_t zero = {0.f, 0.f, 0.f, 0.f};
+
     if (wave < 4) {
-        const int col = slice * 16 + x;   // of the state, of V
+        // ================================================================ the chain
+        const int w = wave, col = slice * 16 + x;
         const bool has_col = col < a.vdim;
         float* st = a.state + ((size_t)span.w * a.H + h) * a.dim_kept * a.vdim;
         f4_t S[OWN][2];
@@ -544,131 +553,171 @@ __global__ __launch_bounds__(512) void k_delta_chunks(DeltaChunks c) {
                     const int d = state_at(j, half) + r;
                     S[j][half][r] = span.z + c.from > 0 && has_col && d < a.dim_kept ? st[(size_t)d * a.vdim + col] : 0.f;
                 }
-        // a chunk's keys of the wave's dims, values and factors of its tokens, T': each asked for when the last chunk's are used
-        u4_t k[OWN][4][W];
-        unsigned v[4];
-        f4_t fa, fc;
-        float fade;
-        b8_t to[2][3];
-        const unsigned v_ld = (unsigned)a.v_ld * ELEM, v_row = has_col ? (16 * w + 4 * g) * v_ld + x * ELEM : NOWHERE;
-        auto fetch_keys = [&](int i) {
-            const auto m = rows_of(a.k, a.k_ld, hq * a.dim, i, a.dim);
-#pragma unroll
-            for (int j = 0; j < OWN; j++) {
-                const int d = 32 * (w + 4 * j) + 8 * g;
-#pragma unroll
-                for (int t = 0; t < 4; t++)
-#pragma unroll
-                    for (int e = 0; e < W; e++) k[j][t][e] = load16(m, d < a.dim ? (unsigned)((16 * t + x) * a.k_ld + d) * ELEM + 16 * e : NOWHERE);
-            }
-        };
-        auto fetch_values = [&](int i) {
-            const auto m = rows_of(a.v, a.v_ld, h * a.vdim + slice * 16, i, min(16, a.vdim - slice * 16));
-#pragma unroll
-            for (int r = 0; r < 4; r++)
-                v[r] = B16 ? (unsigned)__builtin_amdgcn_raw_buffer_load_b16(m, (int)(v_row + r * v_ld), 0, 0) : __builtin_amdgcn_raw_buffer_load_b32(m, (int)(v_row + r * v_ld), 0, 0);
-            fa = __builtin_bit_cast(f4_t, load16(record_of(i), DELTA_OPS + (16 * w + 4 * g) * 4));
-        };
-        auto fetch_factors = [&](int i) {
-            const auto m = record_of(i);
-            fc = __builtin_bit_cast(f4_t, load16(m, DELTA_OPS + (2 * CH + 16 * w + 4 * g) * 4));
-            fade = load4(m, DELTA_OPS + 3 * CH * 4);
-        };
         auto put = [&](u4_t* to, const f4_t& val) {   // [part][64] operands: this tile's half of a lane's eight values
             u2_t parts[3];
             parts_of_four(val, parts);
 #pragma unroll
             for (int p = 0; p < 3; p++) reinterpret_cast<u2_t*>(to + p * 64 + lane)[w & 1] = parts[p];
         };
-        fetch_keys(0);
-        fetch_values(0);
-        fetch_factors(0);
-        fetch_ops(0, 0, to);
+        const unsigned op0 = op_tile(w, 0) * DELTA_TILE + lane * 16, op1 = w >= 2 ? op0 + DELTA_TILE : NOWHERE;   // (no tokens behind the wave's own)
+        b8_t to[2][3];
+        auto fetch_ops = [&](int i) {
+            const auto m = record_of(i);
+#pragma unroll
+            for (int j = 0; j < 3; j++) {
+                to[0][j] = __builtin_bit_cast(b8_t, load16(m, op0 + j * DELTA_PART));
+                to[1][j] = __builtin_bit_cast(b8_t, load16(m, op1 + j * DELTA_PART));
+            }
+        };
+        b8_t k[OWN][4][PARTS];
+        auto keys_of = [&](int i) { return s_k + (L::BUFFERS == 2 ? i & 1 : 0) * DC * PARTS * 256; };
+        auto read_keys = [&](int i, int j) {
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int p = 0; p < PARTS; p++) k[j][t][p] = __builtin_bit_cast(b8_t, keys_of(i)[(((w + 4 * j) * PARTS + p) * CH + 16 * t + x) * 4 + g]);
+        };
+        if (!L::STAGED) fetch_ops(0);
+        __syncthreads();
+        if (L::BUFFERS == 2)
+#pragma unroll
+            for (int j = 0; j < OWN; j++)
+                if (DC % 4 == 0 || w + 4 * j < DC) read_keys(0, j);
         for (int i = 0; i < chunks; i++) {
-            const int next = min(i + 1, chunks - 1);
-            // ---- shares of S^T k
+            // ---- shares of S^T k, each part of the state as soon as it is there
             f4_t D[4] = {zero, zero, zero, zero};
 #pragma unroll
             for (int j = 0; j < OWN; j++) {
                 const int cc = w + 4 * j;
                 if (DC % 4 != 0 && cc >= DC) break;
+                if (L::BUFFERS == 1) read_keys(i, j);
                 b8_t s[3];
-                parts_of_eight(S[j][0], S[j][1], s);
+                if constexpr (B16) {
+                    f4_t lo = S[j][0], hi = S[j][1];
+#pragma unroll
+                    for (int p = 0; p < 3; p++) {
+                        const u2_t l = next_part(lo), u = next_part(hi);
+                        s[p] = __builtin_bit_cast(b8_t, u4_t{l[0], l[1], u[0], u[1]});
+#pragma unroll
+                        for (int t = 0; t < 4; t++) D[t] = mfma(k[j][t][0], s[p], D[t]);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                } else {
+                    parts_of_eight(S[j][0], S[j][1], s);
+#pragma unroll
+                    for (int t = 0; t < 4; t++) D[t] = mfma6(k[j][t], s, D[t]);
+                }
 #pragma unroll
                 for (int p = 0; p < 3; p++) s_S[(cc * 3 + p) * 64 + lane] = __builtin_bit_cast(u4_t, s[p]);
-#pragma unroll
-                for (int t = 0; t < 4; t++) {
-                    b8_t kp[PARTS];
-                    if constexpr (B16) kp[0] = __builtin_bit_cast(b8_t, k[j][t][0]);
-                    else parts_of_eight(__builtin_bit_cast(f4_t, k[j][t][0]), __builtin_bit_cast(f4_t, k[j][t][1]), kp);
-#pragma unroll
-                    for (int p = 0; p < PARTS; p++) s_k[((cc * PARTS + p) * CH + 16 * t + x) * 4 + g] = __builtin_bit_cast(u4_t, kp[p]);
-                    if constexpr (B16) {
-#pragma unroll
-                        for (int p = 2; p >= 0; p--) D[t] = mfma(kp[0], s[p], D[t]);
-                    } else D[t] = mfma6(kp, s, D[t]);
-                }
             }
+            if (DC % 4 != 0) asm volatile("s_nop 15" : "+v"(D[0]), "+v"(D[1]), "+v"(D[2]), "+v"(D[3]));   // (they have come over a branch)
             if (SHARES == 4 || w < SHARES)
 #pragma unroll
                 for (int t = 0; t < 4; t++) s_D[(w * 4 + t) * 64 + lane] = D[t];
-            fetch_keys(next);
             __syncthreads();
-            // ---- X of the wave's tokens
-            f4_t d = s_D[w * 64 + lane];
+            // ---- X of the wave's tokens; T' and factors are read behind the shares, in front of their sums
+            f4_t d[SHARES];
 #pragma unroll
-            for (int j = 1; j < SHARES; j++) d += s_D[(j * 4 + w) * 64 + lane];
-            f4_t X;
+            for (int j = 0; j < SHARES; j++) d[j] = s_D[(j * 4 + w) * 64 + lane];
+            const f4_t fa = *reinterpret_cast<const f4_t*>(s_f + 16 * w + 4 * g);
+            f4_t v;   // tokens 4 g .. + 3 of column x
+            if constexpr (B16) {
+                const u2_t two = __builtin_bit_cast(u2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(reinterpret_cast<unsigned short*>(s_v) + (16 * w + 4 * g + (x >> 2)) * 16 + 4 * (x & 3))));
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const unsigned bits = B16 ? v[r] << 16 : v[r];
-                X[r] = fmaf(-fa[r], d[r], __builtin_bit_cast(float, bits));
+                for (int r = 0; r < 4; r++) {
+                    const unsigned bits = r & 1 ? two[r >> 1] & 0xffff0000u : two[r >> 1] << 16;
+                    v[r] = __builtin_bit_cast(float, bits);
+                }
+            } else {
+#pragma unroll
+                for (int r = 0; r < 4; r++) v[r] = reinterpret_cast<const float*>(s_v)[(16 * w + 4 * g + r) * 16 + x];
             }
+            if (L::STAGED) {
+                get(s_t + op_tile(w, 0) * 192, to[0]);
+                get(s_t + (w >= 2 ? op_tile(w, 1) : 6) * 192, to[1]);   // (no tokens behind the wave's own)
+            }
+            const f4_t fc = *reinterpret_cast<const f4_t*>(s_f + 64 + 16 * w + 4 * g);
+            const float left = s_f[128];
+            __builtin_amdgcn_sched_barrier(0);
+            f4_t X = d[0];
+#pragma unroll
+            for (int j = 1; j < SHARES; j++) X += d[j];
+#pragma unroll
+            for (int r = 0; r < 4; r++) X[r] = fmaf(-fa[r], X[r], v[r]);
             put(s_X + (w >> 1) * 192, X);
-            fetch_values(next);
             __syncthreads();
             // ---- U = T' X
+            // (without a branch for waves 0 and 1: results of the matrix cores that come to their first reader over a branch are not
+            // waited for by the compiler, which left tokens of these waves without their first columns' sums)
             b8_t e[2][3];
             get(s_X, e[0]);
             get(s_X + 192, e[1]);
-            const f4_t U = mfma6(to[0], e[0], zero) + mfma6(to[1], e[1], zero);
-            put(s_V + (w >> 1) * 192, U * fc);
-            put(s_U + (w >> 1) * 192, U);
+            // keys as columns (16 lanes bring 4 tokens x 16 dims, lane x receives dim x of the four), and the next chunk's
+            b8_t kt[OWN][2][2][PARTS];
 #pragma unroll
             for (int j = 0; j < OWN; j++) {
-                S[j][0] *= fade;
-                S[j][1] *= fade;
+                const int cc = w + 4 * j;
+                if (DC % 4 != 0 && cc >= DC) break;
+#pragma unroll
+                for (int half = 0; half < 2; half++)
+#pragma unroll
+                    for (int p = 0; p < 2; p++)
+#pragma unroll
+                        for (int part = 0; part < PARTS; part++) {
+                            const u2_t* at = reinterpret_cast<const u2_t*>(keys_of(i) + ((cc * PARTS + part) * CH + 32 * p + 4 * g + (x >> 2)) * 4 + (x & 3)) + half;
+                            const u2_t lo = __builtin_bit_cast(u2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)at));
+                            const u2_t hi = __builtin_bit_cast(u2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at + 16 * 8)));
+                            kt[j][half][p][part] = __builtin_bit_cast(b8_t, u4_t{lo[0], lo[1], hi[0], hi[1]});
+                        }
+                if (L::BUFFERS == 2) read_keys(i + 1, j);
             }
-            fetch_factors(next);
-            fetch_ops(next, 0, to);
+            __builtin_amdgcn_sched_barrier(0);
+            f4_t U0 = mfma(to[0][1], e[0][1], zero), U1 = mfma(to[0][1], e[0][0], zero), U2 = mfma(to[1][1], e[1][1], zero), U3 = mfma(to[1][1], e[1][0], zero);
+            U0 = mfma(to[0][2], e[0][0], U0);
+            U1 = mfma(to[0][0], e[0][1], U1);
+            U2 = mfma(to[1][2], e[1][0], U2);
+            U3 = mfma(to[1][0], e[1][1], U3);
+            U0 = mfma(to[0][0], e[0][2], U0);
+            U1 = mfma(to[0][0], e[0][0], U1);
+            U2 = mfma(to[1][0], e[1][2], U2);
+            U3 = mfma(to[1][0], e[1][0], U3);
+            const f4_t U = (U0 + U2) + (U1 + U3);
+            put(s_V + (w >> 1) * 192, U * fc);
+#pragma unroll
+            for (int j = 0; j < OWN; j++) {
+                S[j][0] *= left;
+                S[j][1] *= left;
+            }
+            if (!L::STAGED) fetch_ops(i + 1);
             __syncthreads();
-            // ---- the state: keys as columns from LDS (16 lanes bring 4 tokens x 16 dims, lane x receives dim x of the four)
+            // ---- the state
             get(s_V, e[0]);
             get(s_V + 192, e[1]);
 #pragma unroll
             for (int j = 0; j < OWN; j++) {
                 const int cc = w + 4 * j;
                 if (DC % 4 != 0 && cc >= DC) break;
+                if constexpr (B16) {
+                    f4_t more[2] = {zero, zero};
 #pragma unroll
-                for (int half = 0; half < 2; half++) {
+                    for (int part = 0; part < 3; part++)
 #pragma unroll
-                    for (int p = 0; p < 2; p++) {
-                        b8_t kt[PARTS];
-#pragma unroll
-                        for (int part = 0; part < PARTS; part++) {
-                            const u2_t* at = reinterpret_cast<const u2_t*>(s_k + ((cc * PARTS + part) * CH + 32 * p + 4 * g + (x >> 2)) * 4 + (x & 3)) + half;
-                            const u2_t lo = __builtin_bit_cast(u2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)at));
-                            const u2_t hi = __builtin_bit_cast(u2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at + 16 * 8)));
-                            kt[part] = __builtin_bit_cast(b8_t, u4_t{lo[0], lo[1], hi[0], hi[1]});
+                        for (int half = 0; half < 2; half++) {
+                            S[j][half] = mfma(kt[j][half][0][0], e[0][part], S[j][half]);
+                            more[half] = mfma(kt[j][half][1][0], e[1][part], more[half]);
                         }
-                        if constexpr (B16) {
+                    S[j][0] += more[0];
+                    S[j][1] += more[1];
+                } else {
 #pragma unroll
-                            for (int part = 2; part >= 0; part--) S[j][half] = mfma(kt[0], e[p][part], S[j][half]);
-                        } else S[j][half] = mfma6(kt, e[p], S[j][half]);
-                    }
+                    for (int half = 0; half < 2; half++) S[j][half] = mfma6(kt[j][half][1], e[1], mfma6(kt[j][half][0], e[0], S[j][half]));
+                    asm volatile("s_nop 15" : "+v"(S[j][0]), "+v"(S[j][1]));   // (the way round the loop is a branch)
                 }
             }
+            put(s_U + (L::BUFFERS == 2 ? i & 1 : 0) * 384 + (w >> 1) * 192, U);   // (for the results: nobody here waits for it)
+            if (L::BUFFERS == 1) __syncthreads();
         }
+        __syncthreads();   // U is there
 #pragma unroll
         for (int j = 0; j < OWN; j++)
 #pragma unroll
@@ -678,61 +727,222 @@ __global__ __launch_bounds__(512) void k_delta_chunks(DeltaChunks c) {
                     const int d = state_at(j, half) + r;
                     if (has_col && d < a.dim_kept) st[(size_t)d * a.vdim + col] = S[j][half][r];
                 }
-    } else {
-        // ---- results: lane (x, g) has token 16 w + x, columns 4 g .. + 3
-        const unsigned q_row = (16 * w + x) * (unsigned)a.q_ld * ELEM, o_row = ((16 * w + x) * (unsigned)(a.H * a.vdim) + 4 * g) * ELEM;
+    } else if (wave < 6) {
+        // ================================================================ results: lane (x, g) has tokens 16 t + x, columns 4 g .. + 3
+        const int t0 = 2 * (wave - 4);   // token tiles t0, t0 + 1
+        const unsigned o_row = ((16 * t0 + x) * (unsigned)(a.H * a.vdim) + 4 * g) * ELEM, o_tile = 16 * (unsigned)(a.H * a.vdim) * ELEM;
         bool has_out[4];
 #pragma unroll
         for (int e = 0; e < 4; e++) has_out[e] = slice * 16 + 4 * g + e < a.vdim;
-        Rows<DC, B16> q;
-        float fb;
-        b8_t po[2][3];
-        auto fetch_queries = [&](int i) {
-            fb = load4(record_of(i), DELTA_OPS + (CH + 16 * w + x) * 4);
-            q.load(rows_of(a.q, a.q_ld, hq * a.dim, i, a.dim), q_row, a.dim, g);
+        struct Set {
+            Rows<DC, B16> q[2];
+            float fb[2];
+            b8_t po[2][2][3];
         };
-        fetch_queries(0);
-        fetch_ops(0, 1, po);
-        for (int i = 0; i < chunks; i++) {
-            const int next = min(i + 1, chunks - 1);
-            __syncthreads();   // the state is there
-            f4_t O[2] = {zero, zero};
+        constexpr int SETS = sizeof(Set) / 4 <= 84 ? 2 : 1;   // (chunks in flight: what fits the registers)
+        Set set[SETS];
+        auto fetch_queries = [&](Set& s, int i) {
+            const auto m = record_of(i);
+            const auto mq = rows_of(a.q, a.q_ld, hq * a.dim, i, a.dim);
 #pragma unroll
-            for (int cc = 0; cc < DC; cc++) {
-                b8_t s[3], qp[PARTS];
-                get(s_S + cc * 192, s);
-                q.operand(cc, qp);
-                if constexpr (B16) {
-#pragma unroll
-                    for (int p = 2; p >= 0; p--) O[p & 1] = mfma(s[p], qp[0], O[p & 1]);
-                } else O[cc & 1] = mfma6(s, qp, O[cc & 1]);
+            for (int t = 0; t < 2; t++) {
+                s.fb[t] = load4(m, DELTA_OPS + (CH + 16 * (t0 + t) + x) * 4);
+                s.q[t].load(mq, (16 * (t0 + t) + x) * (unsigned)a.q_ld * ELEM, a.dim, g);
             }
-            f4_t o = (O[0] + O[1]) * fb;
-            fetch_queries(next);
-            __syncthreads();
-            __syncthreads();   // U is there
-            b8_t e[2][3];
-            get(s_U, e[0]);
-            get(s_U + 192, e[1]);
-            o = mfma6(e[0], po[0], o) + mfma6(e[1], po[1], zero);
-            fetch_ops(next, 1, po);
-            const auto m = rows_of(a.out, (long)a.H * a.vdim, h * a.vdim + slice * 16, i, min(16, a.vdim - slice * 16));
-            if (c.out_four) {
-                if (B16) __builtin_amdgcn_raw_buffer_store_b64(u2_t{two_b16(o[0], o[1]), two_b16(o[2], o[3])}, m, (int)(has_out[0] ? o_row : NOWHERE), 0, 0);
-                else __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4_t, o), m, (int)(has_out[0] ? o_row : NOWHERE), 0, 0);
-            } else {
+        };
+        auto fetch_ops = [&](Set& s, int i) {
+            const auto m = record_of(i);
 #pragma unroll
-                for (int e1 = 0; e1 < 4; e1++) {
-                    const float y = o[e1];
-                    if (B16) __builtin_amdgcn_raw_buffer_store_b16((unsigned short)two_b16(y, y), m, (int)(has_out[e1] ? o_row + 2 * e1 : NOWHERE), 0, 0);
-                    else __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, y), m, (int)(has_out[e1] ? o_row + 4 * e1 : NOWHERE), 0, 0);
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int p = 0; p < 2; p++)
+#pragma unroll
+                    for (int j = 0; j < 3; j++)
+                        s.po[t][p][j] = __builtin_bit_cast(b8_t, load16(m, p == 0 || t0 > 0 ? (6 + op_tile(t0 + t, p)) * DELTA_TILE + j * DELTA_PART + lane * 16 : NOWHERE));
+        };
+        f4_t o[2];
+        auto finish = [&](const Set& s, int i) {   // chunk i's results: U has come
+            b8_t e[2][3];
+            const u4_t* U = s_U + (L::BUFFERS == 2 ? i & 1 : 0) * 384;
+            get(U, e[0]);
+            get(U + 192, e[1]);
+            const auto m = rows_of(a.out, (long)a.H * a.vdim, h * a.vdim + slice * 16, i, min(16, a.vdim - slice * 16));
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                const f4_t y = mfma6(e[0], s.po[t][0], o[t]) + mfma6(e[1], s.po[t][1], zero);
+                const unsigned at = o_row + t * o_tile;
+                if (c.out_four) {
+                    if (B16) __builtin_amdgcn_raw_buffer_store_b64(u2_t{two_b16(y[0], y[1]), two_b16(y[2], y[3])}, m, (int)(has_out[0] ? at : NOWHERE), 0, 0);
+                    else __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4_t, y), m, (int)(has_out[0] ? at : NOWHERE), 0, 0);
+                } else {
+#pragma unroll
+                    for (int e1 = 0; e1 < 4; e1++) {
+                        const float z = y[e1];
+                        if (B16) __builtin_amdgcn_raw_buffer_store_b16((unsigned short)two_b16(z, z), m, (int)(has_out[e1] ? at + 2 * e1 : NOWHERE), 0, 0);
+                        else __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, z), m, (int)(has_out[e1] ? at + 4 * e1 : NOWHERE), 0, 0);
+                    }
                 }
             }
+        };
+#pragma unroll
+        for (int n = 0; n < SETS; n++) {
+            fetch_queries(set[n], n);
+            fetch_ops(set[n], n);
         }
+        __syncthreads();
+        // (each piece where the chain has as much to do: nobody waits for results)
+        auto step = [&](Set& mine, Set& before, int i) {
+            f4_t O[2][2] = {{zero, zero}, {zero, zero}};
+            auto meet = [&](int c0, int c1) {
+#pragma unroll
+                for (int cc = 0; cc < DC; cc++) {
+                    if (cc < c0 || cc >= c1) continue;
+                    b8_t s[3];
+                    get(s_S + cc * 192, s);
+#pragma unroll
+                    for (int t = 0; t < 2; t++) {
+                        b8_t qp[PARTS];
+                        mine.q[t].operand(cc, qp);
+                        if constexpr (B16) {
+#pragma unroll
+                            for (int p = 2; p >= 0; p--) O[t][p & 1] = mfma(s[p], qp[0], O[t][p & 1]);
+                        } else O[t][cc & 1] = mfma6(s, qp, O[t][cc & 1]);
+                    }
+                }
+            };
+            __syncthreads();   // the state is there, and U of the chunk before
+            meet(0, DC / 2);
+            __syncthreads();
+            meet(DC / 2, DC);
+            f4_t now[2];
+#pragma unroll
+            for (int t = 0; t < 2; t++) now[t] = (O[t][0] + O[t][1]) * mine.fb[t];
+            fetch_queries(mine, i + SETS);
+            __syncthreads();
+            if (L::BUFFERS == 1) __syncthreads();   // U is there
+            if (L::BUFFERS == 2 && i > 0) {
+                finish(before, i - 1);
+                fetch_ops(before, i - 1 + SETS);
+            }
+            o[0] = now[0];
+            o[1] = now[1];
+            if (L::BUFFERS == 1) {
+                finish(mine, i);
+                fetch_ops(mine, i + SETS);
+            }
+        };
+        for (int i = 0; i < chunks; i += SETS) {
+            step(set[0], set[SETS - 1], i);
+            if (SETS == 2 && i + 1 < chunks) step(set[SETS - 1], set[0], i + 1);
+        }
+        __syncthreads();
+        if (L::BUFFERS == 2) {
+            if (SETS == 2 && chunks % 2 == 0) finish(set[SETS - 1], chunks - 1);
+            else finish(set[0], chunks - 1);
+        }
+    } else {
+        // ================================================================ keys, values, T' and factors on their way to LDS
+        const int tid = threadIdx.x - 384;   // of 128
+        constexpr int ROW = DC <= 1 ? 4 : DC <= 2 ? 8 : DC <= 4 ? 16 : 32, ITEMS = CH * ROW / 128, W = B16 ? 1 : 2;   // a row's pieces of 8 dims, rounded up
+        const int piece = tid % ROW, row = tid / ROW;   // items: tokens row + i * (128 / ROW)
+        const bool has_piece = piece < 4 * DC;
+        const unsigned k_at = 8 * piece < a.dim ? ((unsigned)row * (unsigned)a.k_ld + 8 * piece) * ELEM : NOWHERE, k_step = (128 / ROW) * (unsigned)a.k_ld * ELEM;
+        // 16 bytes of a token's 16 values: thread 2 t (+ 1) of token t, in 32 bits 4 t' .. + 3 of tokens t' and 32 + t'
+        const int v_col = slice * 16 + (B16 ? 8 * (tid & 1) : 4 * (tid & 3));
+        const unsigned v_ld = (unsigned)a.v_ld * ELEM, v_at = v_col < a.v_cols ? (B16 ? (tid >> 1) * v_ld + 16 * (tid & 1) : (tid >> 2) * v_ld + 16 * (tid & 3)) : NOWHERE;
+        const unsigned f_at = tid < 16 ? DELTA_OPS + tid * 16 : tid < 32 ? DELTA_OPS + 2 * CH * 4 + (tid - 16) * 16 : tid == 32 ? DELTA_OPS + 3 * CH * 4 : NOWHERE;
+        struct Set {
+            u4_t k[ITEMS][W], t[L::STAGED ? 9 : 1], f, v[W];
+        };
+        constexpr int SETS = sizeof(Set) / 4 <= 88 ? 2 : 1;   // (chunks in flight: what fits the registers)
+        Set set[SETS];
+        auto fetch_keys = [&](Set& s, int i) {
+            const auto m = rows_of(a.k, a.k_ld, hq * a.dim, i, a.dim);
+#pragma unroll
+            for (int n = 0; n < ITEMS; n++)
+#pragma unroll
+                for (int e = 0; e < W; e++) s.k[n][e] = load16(m, k_at + n * k_step + 16 * e);
+        };
+        auto fetch_values = [&](Set& s, int i) {
+            const auto m = rows_of(a.v, a.v_ld, h * a.v_cols + slice * 16, i, min(16, a.v_cols - slice * 16));
+#pragma unroll
+            for (int e = 0; e < W; e++) s.v[e] = load16(m, v_at + 32 * e * v_ld);
+        };
+        auto fetch_ops = [&](Set& s, int i) {
+            const auto m = record_of(i);
+            if (L::STAGED)
+#pragma unroll
+                for (int n = 0; n < 9; n++) s.t[n] = load16(m, (n * 128 + tid) * 16);
+            s.f = load16(m, f_at);
+        };
+        auto lay_keys = [&](const Set& s, int i) {
+            u4_t* keys = s_k + (L::BUFFERS == 2 ? i & 1 : 0) * DC * PARTS * 256 + (piece >> 2) * PARTS * 256 + row * 4 + (piece & 3);
+#pragma unroll
+            for (int n = 0; n < ITEMS; n++) {
+                b8_t p[PARTS];
+                if constexpr (B16) p[0] = __builtin_bit_cast(b8_t, s.k[n][0]);
+                else parts_of_eight(__builtin_bit_cast(f4_t, s.k[n][0]), __builtin_bit_cast(f4_t, s.k[n][1]), p);
+                if (has_piece)
+#pragma unroll
+                    for (int j = 0; j < PARTS; j++) keys[j * 256 + n * (128 / ROW) * 4] = __builtin_bit_cast(u4_t, p[j]);
+            }
+        };
+        auto lay_values = [&](const Set& s) {
+#pragma unroll
+            for (int e = 0; e < W; e++) s_v[tid + 128 * e] = s.v[e];
+            if (tid < 16) reinterpret_cast<u4_t*>(s_f)[tid] = s.f;
+        };
+        auto lay_ops = [&](const Set& s) {
+            if (L::STAGED)
+#pragma unroll
+                for (int n = 0; n < 9; n++) s_t[n * 128 + tid] = s.t[n];
+            if (tid >= 16 && tid <= 32) reinterpret_cast<u4_t*>(s_f)[tid] = s.f;
+        };
+        auto fetch = [&](Set& s, int i) {
+            fetch_keys(s, i);
+            fetch_values(s, i);
+            fetch_ops(s, i);
+        };
+        fetch(set[0], 0);
+        if (SETS == 2) fetch(set[1], 1);
+        lay_keys(set[0], 0);
+        lay_values(set[0]);
+        lay_ops(set[0]);
+        if (L::STAGED) {
+            s_t[6 * 192 + tid] = u4_t{0, 0, 0, 0};
+            if (tid < 64) s_t[6 * 192 + 128 + tid] = u4_t{0, 0, 0, 0};
+        }
+        fetch(set[0], SETS);
+        __syncthreads();
+        auto step = [&](Set& s, int i) {   // while chunk i is computed: chunk i + 1 to LDS, the one that is SETS behind it is asked for
+            const int then = i + 1 + SETS;
+            __syncthreads();
+            if (L::BUFFERS == 2) {
+                lay_keys(s, i + 1);
+                fetch_keys(s, then);
+            }
+            __syncthreads();
+            lay_values(s);
+            fetch_values(s, then);
+            __syncthreads();
+            if (L::BUFFERS == 1) {
+                lay_keys(s, i + 1);
+                fetch_keys(s, then);
+            }
+            lay_ops(s);
+            fetch_ops(s, then);
+            if (L::BUFFERS == 1) __syncthreads();
+        };
+        for (int i = 0; i < chunks; i += SETS) {
+            step(set[SETS - 1], i);
+            if (SETS == 2 && i + 1 < chunks) step(set[0], i + 1);
+        }
+        __syncthreads();
     }
 }
 
 // Rows of queries and keys whose dims or addresses the chunk kernels' loads do not fit: dims padded to a multiple of 8 with zeros.
+// (The same for values.)
 template <typename E>
 __global__ __launch_bounds__(256) void k_delta_rows(E* __restrict__ dst, const E* __restrict__ src, int Q, int dim, int dim_ld, long ld) {
     const long row = blockIdx.x;
@@ -745,7 +955,7 @@ __global__ __launch_bounds__(256) void k_delta_rows(E* __restrict__ dst, const E
 template <int DC, bool B16>
 static void launch_chunks_of(const DeltaChunks& c) {
     const Delta& a = c.a;
-    constexpr int prep = prepare_lds<DC, B16>(), walk = chunks_lds<DC, B16>();
+    constexpr int prep = prepare_lds<DC, B16>(), walk = Walk<DC, B16>::LDS;
     static bool enabled = false;
     if (!enabled) {
         HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(&k_delta_prepare<DC, B16>), hipFuncAttributeMaxDynamicSharedMemorySize, prep));
@@ -856,23 +1066,30 @@ static int gated_delta(Delta& a, const int* seq_ids, const int* pos, int T, int 
         c.out_four = a.vdim % 4 == 0 && (size_t)a.out % (4 * elem) == 0;
         size_t n_records = 0;
         for (int i = 0; i < n_chunked; i++) n_records = std::max(n_records, (size_t)first[i] + std::min(most, cdiv(spans[i].y, CH)));
-        const int per16 = 16 / elem, dim_ld = (a.dim + 7) & ~7;
+        const int per16 = 16 / elem, dim_ld = (a.dim + 7) & ~7, vdim_ld = (a.vdim + 7) & ~7;
         const bool fits = a.dim % 8 == 0 && a.q_ld % per16 == 0 && a.k_ld % per16 == 0 && ((size_t)a.q | (size_t)a.k) % 16 == 0;
-        const size_t rows = fits ? 0 : (size_t)T * a.Q * dim_ld * elem;
-        const size_t row_room = (rows + 255) & ~(size_t)255;
-        char* mem = (char*)ws_get(WS_DELTA, 2 * row_room + n_records * a.H * DELTA_RECORD);
+        const bool v_fits = a.vdim % per16 == 0 && a.v_ld % per16 == 0 && (size_t)a.v % 16 == 0;
+        auto room = [&](bool needed, int heads, int ld) { return needed ? ((size_t)T * heads * ld * elem + 255) & ~(size_t)255 : 0; };
+        const size_t qk_room = room(!fits, a.Q, dim_ld), v_room = room(!v_fits, a.H, vdim_ld);
+        char* mem = (char*)ws_get(WS_DELTA, 2 * qk_room + v_room + n_records * a.H * DELTA_RECORD);
+        auto pack = [&](const void*& src, long& ld, int heads, int dim, int wide) {
+            if (b16) NVLLM_LAUNCH((k_delta_rows<unsigned short>), dim3(T), dim3(256), 0, (unsigned short*)mem, (const unsigned short*)src, heads, dim, wide, ld);
+            else NVLLM_LAUNCH((k_delta_rows<float>), dim3(T), dim3(256), 0, (float*)mem, (const float*)src, heads, dim, wide, ld);
+            src = mem;
+            ld = (long)heads * wide;
+        };
+        c.a.v_cols = a.vdim;
         if (!fits) {
-            auto pack = [&](const void* src, long ld, char* dst) {
-                if (b16) NVLLM_LAUNCH((k_delta_rows<unsigned short>), dim3(T), dim3(256), 0, (unsigned short*)dst, (const unsigned short*)src, a.Q, a.dim, dim_ld, ld);
-                else NVLLM_LAUNCH((k_delta_rows<float>), dim3(T), dim3(256), 0, (float*)dst, (const float*)src, a.Q, a.dim, dim_ld, ld);
-            };
-            pack(a.q, a.q_ld, mem);
-            pack(a.k, a.k_ld, mem + row_room);
-            c.a.q = mem;
-            c.a.k = mem + row_room;
-            c.a.q_ld = c.a.k_ld = (long)a.Q * dim_ld;
+            pack(c.a.q, c.a.q_ld, a.Q, a.dim, dim_ld);
+            mem += qk_room;
+            pack(c.a.k, c.a.k_ld, a.Q, a.dim, dim_ld);
+            mem += qk_room;
             c.a.dim = dim_ld;
-            mem += 2 * row_room;
+        }
+        if (!v_fits) {
+            pack(c.a.v, c.a.v_ld, a.H, a.vdim, vdim_ld);
+            mem += v_room;
+            c.a.v_cols = vdim_ld;
         }
         c.mem = mem;
         // the algorithm's bytes and flops, split over the launches
