@@ -232,7 +232,30 @@ __device__ __forceinline__ f4_t mfma6(const b8_t (&a)[3], const b8_t (&b)[3], f4
     return mfma(a[0], b[0], c);
 }
 __device__ __forceinline__ f4_t mfma4(float a, float b, const f4_t& c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
-__device__ __forceinline__ float exp_of(double x) { return __builtin_amdgcn_exp2f((float)(x * 1.4426950408889634)); }
+// Sums of g in units of log2(e): two floats, so that differences of neighbouring tokens' keep 32 bits however far the sums have come.
+struct Sum2 {
+    float hi, lo;
+};
+__device__ __forceinline__ float exp_of(const Sum2& a, const Sum2& b) { return __builtin_amdgcn_exp2f((a.hi - b.hi) + (a.lo - b.lo)); }
+template <int CTRL>
+__device__ __forceinline__ double from_lane(double x) {   // zeros from outside the row of lanes
+    const long v = __builtin_bit_cast(long, x);
+    const int lo = __builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true), hi = __builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, 0xf, 0xf, true);
+    return __builtin_bit_cast(double, (long)(unsigned)lo | (long)hi << 32);
+}
+__device__ __forceinline__ double scalar_of(double x, int lane) {
+    const long v = __builtin_bit_cast(long, x);
+    return __builtin_bit_cast(double, (long)(unsigned)__builtin_amdgcn_readlane((int)v, lane) | (long)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32);
+}
+// the sum over the wave's lanes up to this one
+__device__ __forceinline__ double sum_up_to(double x, int lane) {
+    x += from_lane<0x111>(x);   // row_shr:1, 2, 4, 8
+    x += from_lane<0x112>(x);
+    x += from_lane<0x114>(x);
+    x += from_lane<0x118>(x);
+    const double r0 = scalar_of(x, 15), r1 = r0 + scalar_of(x, 31), r2 = r1 + scalar_of(x, 47);
+    return x + (lane < 16 ? 0.0 : lane < 32 ? r0 : lane < 48 ? r1 : r2);
+}
 
 // Memory by descriptors: what lies behind `bytes` (and every offset of NOWHERE) reads as zeros and is not written, so that a chunk's
 // loads have no branch around them and all of them are in flight together.
@@ -248,17 +271,6 @@ template <int DC, bool B16>
 struct Rows {
     static constexpr int W = B16 ? 1 : 2;
     u4_t w[DC][W];
-    __device__ __forceinline__ void load(const void* base, size_t row, int dim, int g, bool there) {
-#pragma unroll
-        for (int cc = 0; cc < DC; cc++) {
-            const int d = 32 * cc + 8 * g;
-#pragma unroll
-            for (int i = 0; i < W; i++) {
-                w[cc][i] = u4_t{0, 0, 0, 0};
-                if (there && d < dim) w[cc][i] = *reinterpret_cast<const u4_t*>((const char*)base + (row + d) * (B16 ? 2 : 4) + 16 * i);
-            }
-        }
-    }
     // row: the offset of a token's row in bytes
     __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t m, unsigned row, int dim, int g) {
 #pragma unroll
@@ -322,17 +334,20 @@ __device__ __forceinline__ ChunkAt chunk_at(const DeltaChunks& c, int s, int h, 
 __device__ __forceinline__ int op_tile(int w, int p) { return w < 2 ? w : 2 * w - 2 + p; }
 
 constexpr int LD = CH + 4;   // floats of a row of A or T in LDS
+// keys as operands, in whose place T comes later; A; sums of g, what norms a key, beta
 template <int DC, bool B16>
-constexpr int prepare_lds() { return 4 * DC * (B16 ? 1 : 3) * 1024 + 2 * CH * LD * 4 + CH * (8 + 4 + 4); }
+constexpr int prepare_keys() { return std::max(4 * DC * (B16 ? 1 : 3) * 1024, CH * LD * 4); }
+template <int DC, bool B16>
+constexpr int prepare_lds() { return prepare_keys<DC, B16>() + CH * LD * 4 + CH * (8 + 4 + 4); }
 
 template <int DC, bool B16>
 __global__ __launch_bounds__(256) void k_delta_prepare(DeltaChunks c) {
     constexpr int PARTS = B16 ? 1 : 3;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds_d[];
     u4_t* s_k = reinterpret_cast<u4_t*>(lds_d);                            // [token tile][DC][part][64]
-    float* s_A = reinterpret_cast<float*>(s_k + 4 * DC * PARTS * 64);      // [t][LD]
-    float* s_T = s_A + CH * LD;
-    double* s_G = reinterpret_cast<double*>(s_T + CH * LD);
+    float* s_T = reinterpret_cast<float*>(lds_d);                          // [t][LD]
+    float* s_A = reinterpret_cast<float*>(lds_d + prepare_keys<DC, B16>());
+    Sum2* s_G = reinterpret_cast<Sum2*>(s_A + CH * LD);
     float* s_r = reinterpret_cast<float*>(s_G + CH);                       // what norms a key
     float* s_b = s_r + CH;
     const Delta& a = c.a;
@@ -341,21 +356,18 @@ __global__ __launch_bounds__(256) void k_delta_prepare(DeltaChunks c) {
     if (at.n <= 0) return;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), x = lane & 15, g = lane >> 4;
     const int t = 16 * w + x;
+    constexpr int ELEM = B16 ? 2 : 4;
     Rows<DC, B16> k, q;
-    const bool there = t < at.n;
-    k.load(a.k, (size_t)(at.first + t) * a.k_ld + hq * a.dim, a.dim, g, there);
-    q.load(a.q, (size_t)(at.first + t) * a.q_ld + hq * a.dim, a.dim, g, there);
+    auto rows_of = [&](const void* base, long ld) { return memory((const char*)base + ((size_t)at.first * ld + hq * a.dim) * ELEM, ((at.n - 1) * ld + a.dim) * ELEM); };
+    const auto gates = [&](const float* base) { return load4(memory(base + (size_t)at.first * a.H + h, ((long)(at.n - 1) * a.H + 1) * 4), (unsigned)lane * a.H * 4); };
+    const float gl = gates(a.g), bl = gates(a.beta);   // (zeros behind the last token)
+    k.load(rows_of(a.k, a.k_ld), (unsigned)t * (unsigned)a.k_ld * ELEM, a.dim, g);
+    q.load(rows_of(a.q, a.q_ld), (unsigned)t * (unsigned)a.q_ld * ELEM, a.dim, g);
     if (w == 0) {
-        const size_t i = (size_t)(at.first + min(lane, at.n - 1)) * a.H + h;
-        const float gl = a.g[i];
-        double G = lane < at.n ? (double)(gl < MIN_G ? MIN_G : gl) : 0.0;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const double before = __shfl_up(G, o, 64);
-            if (lane >= o) G += before;
-        }
-        s_G[lane] = G;
-        s_b[lane] = lane < at.n ? a.beta[i] : 0.f;
+        const double G = sum_up_to((double)(gl < MIN_G ? MIN_G : gl) * 1.4426950408889634, lane);
+        const float hi = (float)G;
+        s_G[lane] = Sum2{hi, (float)(G - (double)hi)};
+        s_b[lane] = bl;
     }
     float rk = 1.f, rq = 1.f;
     if (a.eps > 0.f) {
@@ -378,7 +390,7 @@ __global__ __launch_bounds__(256) void k_delta_prepare(DeltaChunks c) {
     }
     __syncthreads();
     // rows s of tile i, columns t of tile w
-    const double Gt = s_G[t];
+    const Sum2 Gt = s_G[t], none = {0.f, 0.f};
     const float bt = s_b[t] * rk, qt = a.scale * rq;
     f4_t kq[4];
 #pragma unroll
@@ -397,7 +409,7 @@ __global__ __launch_bounds__(256) void k_delta_prepare(DeltaChunks c) {
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 const int s = 16 * i + 4 * g + r;
-                const float f = exp_of(Gt - s_G[s]) * s_r[s];   // (not used where s lies behind t)
+                const float f = exp_of(Gt, s_G[s]) * s_r[s];   // (not used where s lies behind t)
                 kk[r] = s < t ? bt * f * kk[r] : 0.f;
                 kq[i][r] = s <= t ? qt * f * kq[i][r] : 0.f;
             }
@@ -416,53 +428,61 @@ __global__ __launch_bounds__(256) void k_delta_prepare(DeltaChunks c) {
     if (threadIdx.x < CH) {   // (wave 0: t is not this thread's token)
         float* f = reinterpret_cast<float*>(at.record + DELTA_OPS);
         const int tok = threadIdx.x;
-        f[tok] = exp_of(s_G[tok]) * s_r[tok];
-        f[2 * CH + tok] = exp_of(s_G[CH - 1] - s_G[tok]) * s_r[tok];
-        if (tok == 0) f[3 * CH] = exp_of(s_G[CH - 1]);
+        f[tok] = exp_of(s_G[tok], none) * s_r[tok];
+        f[2 * CH + tok] = exp_of(s_G[CH - 1], s_G[tok]) * s_r[tok];
+        if (tok == 0) f[3 * CH] = exp_of(s_G[CH - 1], none);
     }
-    if (g == 0) reinterpret_cast<float*>(at.record + DELTA_OPS)[CH + t] = qt * exp_of(Gt);
+    if (g == 0) reinterpret_cast<float*>(at.record + DELTA_OPS)[CH + t] = qt * exp_of(Gt, none);
     __syncthreads();
-    // (I + A)^-1: wave w first its block on the diagonal, a lane a column ...
-    {
+    // (I + A)^-1: first the four blocks on the diagonal, by one wave: lane (x, g) has column x of block g, and row x of its A, whose
+    // values the row of lanes shares (by a fused move; one LDS read after the other took 7,000 clocks, scalars 2,800).
+    if (w == 0) {
+        f4_t A[4];
         float col[16];
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            float v = i == x ? 1.f : 0.f;
+        for (int i = 0; i < 4; i++) A[i] = *reinterpret_cast<const f4_t*>(s_A + (16 * g + x) * LD + 16 * g + 4 * i);
 #pragma unroll
-            for (int s4 = 0; s4 < (i + 3) / 4; s4++) {
-                const f4_t A = *reinterpret_cast<const f4_t*>(s_A + (16 * w + i) * LD + 16 * w + 4 * s4);
+        for (int i = 0; i < 16; i++) col[i] = i == x ? 1.f : 0.f;
+        // (row_newbcast: the value of lane i of each row of lanes)
+#define COLUMN_STEP(S, I) \
+    if (I > S) col[I] = fmaf(-__builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, as), 0x150 + I, 0xf, 0xf, true)), col[S], col[I]);
+#define COLUMN(S)                                                                                                                                       \
+    {                                                                                                                                                   \
+        const float as = A[S / 4][S % 4];                                                                                                               \
+        COLUMN_STEP(S, 1) COLUMN_STEP(S, 2) COLUMN_STEP(S, 3) COLUMN_STEP(S, 4) COLUMN_STEP(S, 5) COLUMN_STEP(S, 6) COLUMN_STEP(S, 7) COLUMN_STEP(S, 8) \
+        COLUMN_STEP(S, 9) COLUMN_STEP(S, 10) COLUMN_STEP(S, 11) COLUMN_STEP(S, 12) COLUMN_STEP(S, 13) COLUMN_STEP(S, 14) COLUMN_STEP(S, 15)             \
+    }
+        COLUMN(0) COLUMN(1) COLUMN(2) COLUMN(3) COLUMN(4) COLUMN(5) COLUMN(6) COLUMN(7) COLUMN(8) COLUMN(9) COLUMN(10) COLUMN(11) COLUMN(12) COLUMN(13) COLUMN(14)
+#undef COLUMN
+#undef COLUMN_STEP
 #pragma unroll
-                for (int s = 4 * s4; s < i && s < 4 * s4 + 4; s++) v = fmaf(-A[s & 3], col[s], v);
-            }
-            col[i] = v;
-        }
-        if (g == 0)
-#pragma unroll
-            for (int i = 0; i < 16; i++) s_T[(16 * w + i) * LD + 16 * w + x] = col[i];
+        for (int i = 0; i < 16; i++) s_T[(16 * g + i) * LD + 16 * g + x] = col[i];
     }
     __syncthreads();
-    // ... then the blocks under it, from the top: T_iw = -T_ii sum_j A_ij T_jw.  (k of these products runs 4 g + step, as results lie)
+    // ... then the blocks under it, block column w by wave w, from the top: T_iw = -T_ii sum_j A_ij T_jw, every T_jw added to all sums
+    // below as soon as it is there.  (k of these products runs 4 g + step, as results lie)
     {
-        f4_t T[4];
+        f4_t T, sum[4] = {};
 #pragma unroll
-        for (int r = 0; r < 4; r++) T[0][r] = s_T[(16 * w + 4 * g + r) * LD + 16 * w + x];
+        for (int r = 0; r < 4; r++) T[r] = s_T[(16 * w + 4 * g + r) * LD + 16 * w + x];
 #pragma unroll
-        for (int j = 1; j < 4; j++) {
-            const int i = w + j;
-            if (i >= 4) break;
-            f4_t sum = {0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < 3; j++) {
+            if (w + j >= 3) break;
 #pragma unroll
-            for (int m = 0; m < j; m++) {
-                const f4_t A = *reinterpret_cast<const f4_t*>(s_A + (16 * i + x) * LD + 16 * (w + m) + 4 * g);
+            for (int i = j + 1; i < 4; i++) {
+                if (w + i >= 4) break;
+                const f4_t A = *reinterpret_cast<const f4_t*>(s_A + (16 * (w + i) + x) * LD + 16 * (w + j) + 4 * g);
 #pragma unroll
-                for (int e = 0; e < 4; e++) sum = mfma4(A[e], T[m][e], sum);
+                for (int e = 0; e < 4; e++) sum[i] = mfma4(A[e], T[e], sum[i]);
             }
-            const f4_t D = *reinterpret_cast<const f4_t*>(s_T + (16 * i + x) * LD + 16 * i + 4 * g);
-            T[j] = f4_t{0.f, 0.f, 0.f, 0.f};
+            asm volatile("s_nop 15" : "+v"(sum[j + 1]));   // (it has come over a branch)
+            const int row = 16 * (w + j + 1);
+            const f4_t D = *reinterpret_cast<const f4_t*>(s_T + (row + x) * LD + row + 4 * g);
+            T = f4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int e = 0; e < 4; e++) T[j] = mfma4(-D[e], sum[e], T[j]);
+            for (int e = 0; e < 4; e++) T = mfma4(-D[e], sum[j + 1][e], T);
 #pragma unroll
-            for (int r = 0; r < 4; r++) s_T[(16 * i + 4 * g + r) * LD + 16 * w + x] = T[j][r];
+            for (int r = 0; r < 4; r++) s_T[(row + 4 * g + r) * LD + 16 * w + x] = T[r];
         }
     }
     __syncthreads();
