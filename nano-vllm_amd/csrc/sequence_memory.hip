@@ -16,10 +16,12 @@ bool stream_is_captured() {
 }
 
 // ------------------------------------------------------------------ the copy
-// A program is a list of moves (slot, slot) that a thread makes for its own bytes of a slot, one after the other, in every array
-// alike: no thread touches another's bytes, so programs with different slots need no order, and a cycle of slots is one
-// program with a value set aside (slot -1).  Moves that share a source read it once.
-constexpr int COPY_SETS = 6, COPY_INLINE = 200, COPY_FAN = 4;
+// A program is a list of moves (slot, slot) that a thread makes for its own bytes of a slot, in every array alike: no thread
+// touches another's bytes, so programs with different slots need no order, and a cycle of slots is one program with a value set
+// aside (slot -1).  A slot is written after its last reading, so the readings of four moves are in flight before the first of
+// their writes.  Moves that share a source read it once.  Bound by memory: 369 MB take 74 us where a copy of 1 GiB reaches 5.1 TB/s, and
+// by the launch and three trips to memory behind one another where there is little to copy.
+constexpr int COPY_SETS = 6, COPY_INLINE = 200, COPY_FAN = 4, COPY_BATCH = 4;
 struct CopySet {
     char* base;
     size_t stride;
@@ -28,47 +30,59 @@ struct CopySet {
 };
 struct CopyArgs {
     CopySet sets[COPY_SETS];
-    int n_sets, n_programs;
+    int n_programs;
     const int* programs;          // null: the ints are right here
     int here[COPY_INLINE];        // [n_programs + 1] first moves, then moves (from, to)
 };
 
-template <typename U, int N>
+template <typename U, int N, bool HERE>
 __global__ __launch_bounds__(256) void k_copy_slots(CopyArgs a) {
     const int array = blockIdx.y, program = blockIdx.x % a.n_programs;
     const unsigned first = (blockIdx.x / a.n_programs) * (256 * N) + threadIdx.x;
-    int set = 0;
-    while (set + 1 < a.n_sets && array >= a.sets[set + 1].first) set++;
-    const unsigned units = a.sets[set].units;
-    if (first >= units) return;
-    U* base = reinterpret_cast<U*>(a.sets[set].base + (size_t)(array - a.sets[set].first) * a.sets[set].stride);
-    const int* prog = a.programs ? a.programs : a.here;
-    const int begin = prog[program], end = prog[program + 1];
-    const int* moves = prog + a.n_programs + 1;
-    U now[N] = {}, aside[N] = {};
-    int have = -2;
-    for (int m = begin; m < end; m++) {
-        const int from = moves[2 * m], to = moves[2 * m + 1];
-        if (from != have) {
-            if (from < 0) {
+    CopySet set = a.sets[0];
 #pragma unroll
-                for (int i = 0; i < N; i++) now[i] = aside[i];
+    for (int i = 1; i < COPY_SETS; i++)   // (sets that are not there begin behind the last array)
+        if (array >= a.sets[i].first) set = a.sets[i];
+    if (first >= set.units) return;
+    U* base = reinterpret_cast<U*>(set.base + (size_t)(array - set.first) * set.stride);
+    auto number = [&](int i) { return __builtin_amdgcn_readfirstlane(HERE ? a.here[i] : a.programs[i]); };
+    const int begin = number(program), end = number(program + 1), moves = a.n_programs + 1;
+    U aside[N] = {};
+    for (int m = begin; m < end; m += COPY_BATCH) {
+        int from[COPY_BATCH], to[COPY_BATCH];
+#pragma unroll
+        for (int j = 0; j < COPY_BATCH; j++) {   // (behind the last move: the last one)
+            from[j] = number(moves + 2 * min(m + j, end - 1));
+            to[j] = number(moves + 2 * min(m + j, end - 1) + 1);
+        }
+        U v[COPY_BATCH][N] = {};
+#pragma unroll
+        for (int j = 0; j < COPY_BATCH; j++) {
+            if (m + j >= end) break;
+            if (from[j] < 0) {
+#pragma unroll
+                for (int i = 0; i < N; i++) v[j][i] = aside[i];
+            } else if (j > 0 && from[j] == from[j - 1]) {
+#pragma unroll
+                for (int i = 0; i < N; i++) v[j][i] = v[j - 1][i];
             } else {
-                const U* s = base + (size_t)from * units;
+                const U* s = base + (size_t)from[j] * set.units;
 #pragma unroll
                 for (int i = 0; i < N; i++)
-                    if (first + 256 * i < units) now[i] = s[first + 256 * i];
+                    if (first + 256 * i < set.units) v[j][i] = s[first + 256 * i];
             }
-            have = from;
-        }
-        if (to < 0) {
+            if (to[j] < 0)
 #pragma unroll
-            for (int i = 0; i < N; i++) aside[i] = now[i];
-        } else {
-            U* d = base + (size_t)to * units;
+                for (int i = 0; i < N; i++) aside[i] = v[j][i];
+        }
+#pragma unroll
+        for (int j = 0; j < COPY_BATCH; j++) {
+            if (m + j >= end) break;
+            if (to[j] < 0) continue;
+            U* d = base + (size_t)to[j] * set.units;
 #pragma unroll
             for (int i = 0; i < N; i++)
-                if (first + 256 * i < units) d[first + 256 * i] = now[i];
+                if (first + 256 * i < set.units) d[first + 256 * i] = v[j][i];
         }
     }
 }
@@ -198,7 +212,9 @@ template <typename U>
 static void launch_copy(const CopyArgs& a, unsigned most_units, int arrays) {
     constexpr int N = 2;
     const long pieces = (most_units + 256 * N - 1) / (256 * N);
-    NVLLM_LAUNCH((k_copy_slots<U, N>), dim3((unsigned)(pieces * a.n_programs), arrays), dim3(256), 0, a);
+    const dim3 grid((unsigned)(pieces * a.n_programs), arrays);
+    if (a.programs) NVLLM_LAUNCH((k_copy_slots<U, N, false>), grid, dim3(256), 0, a);
+    else NVLLM_LAUNCH((k_copy_slots<U, N, true>), grid, dim3(256), 0, a);
 }
 
 int copy_slots(const std::vector<SlotArrays>& arrays, int n_slots, const int* from, const int* to, int n) {
@@ -229,18 +245,18 @@ int copy_slots(const std::vector<SlotArrays>& arrays, int n_slots, const int* fr
         a.programs = dev;
     }
     for (size_t i = 0; i < arrays.size();) {
-        int total = 0;
+        int total = 0, sets = 0;
         unsigned most = 0;
         double part = 0;
-        a.n_sets = 0;
-        for (; i < arrays.size() && a.n_sets < COPY_SETS && total + arrays[i].count <= 65535; i++) {
+        for (; i < arrays.size() && sets < COPY_SETS && total + arrays[i].count <= 65535; i++) {
             const SlotArrays& s = arrays[i];
             if (s.count == 0 || s.slot_bytes == 0) continue;
-            a.sets[a.n_sets++] = CopySet{(char*)s.base, s.stride, (unsigned)(s.slot_bytes / unit), total};
+            a.sets[sets++] = CopySet{(char*)s.base, s.stride, (unsigned)(s.slot_bytes / unit), total};
             most = std::max(most, (unsigned)(s.slot_bytes / unit));
             part += 2.0 * n * (double)s.slot_bytes * s.count;
             total += s.count;
         }
+        for (int j = sets; j < COPY_SETS; j++) a.sets[j] = CopySet{nullptr, 0, 0, 0x7fffffff};
         if (total == 0) continue;
         ProfScope ps(PC_SLOT_COPY, part, 0);
         if (unit == 16) launch_copy<uint4>(a, most, total);
