@@ -35,6 +35,9 @@ struct DeltaChunks {
     const int* first;           // [n_spans] the launch's first chunk of each span; null: the ones here
     int first_here[DELTA_SPANS];
     int from, most;             // chunks [from, from + most) of every span
+    int segs, per_seg;          // segments of a portion's chunks of the launch at most, chunks of one
+    float* starts;              // [span][segs][H][dims][columns] states that segments start from, both padded (see k_delta_walk) ...
+    float* trans;               // [span][segs][H][dims][dims] ... and what becomes of a state over a segment
     bool out_four;              // out can be stored four elements at a time
     double bytes, flops;        // kernel timing
 };

@@ -514,6 +514,10 @@ __global__ __launch_bounds__(256) void k_delta_prepare(DeltaChunks c) {
 //   6, 7 bring keys, values, T' and factors of coming chunks from memory, one or two chunks ahead, and lay them out in LDS: the chain
 //     itself asks memory for nothing.
 // Three barriers a chunk (a fourth where LDS holds one chunk's keys only).
+//
+// A portion's chunks may be cut into segments that are walked side by side: scouts (RESULTS false) find out what a segment makes of an empty
+// state (the first one: of the portion's) and, for columns of the unit matrix, what becomes of a state over it, k_delta_join forms the
+// states that segments start from, and they are walked from there.
 template <int DC, bool B16>
 struct Walk {
     static constexpr int PARTS = B16 ? 1 : 3;
@@ -524,7 +528,7 @@ struct Walk {
     static constexpr int LDS = REST + (BUFFERS - 1) * EX + BUFFERS * KEYS + (STAGED ? OPS : 0);
 };
 
-template <int DC, bool B16>
+template <int DC, bool B16, bool RESULTS>
 __global__ __launch_bounds__(512) void k_delta_chunks(DeltaChunks c) {
     typedef Walk<DC, B16> L;
     constexpr int PARTS = L::PARTS, OWN = (DC + 3) / 4, SHARES = DC < 4 ? DC : 4, ELEM = B16 ? 2 : 4;
@@ -539,13 +543,16 @@ __global__ __launch_bounds__(512) void k_delta_chunks(DeltaChunks c) {
     u4_t* s_k = reinterpret_cast<u4_t*>(s_f + 256);        // [buffer][DC][part][token][4] keys, 32 dims together
     u4_t* s_t = s_k + L::BUFFERS * DC * PARTS * 256;       // T', and a tile of zeros
     const Delta& a = c.a;
-    const int h = blockIdx.x, slice = blockIdx.y, hq = h / (a.H / a.Q);
+    const int h = blockIdx.x, hq = h / (a.H / a.Q), of = blockIdx.z / c.segs, seg = blockIdx.z - of * c.segs;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), x = lane & 15, g = lane >> 4;
-    const int4 span = span_of(a, blockIdx.z);
-    const int chunks = min(c.most, (span.y + CH - 1) / CH - c.from);
-    if (chunks <= 0) return;
-    const int first = span.x + c.from * CH, tokens = min(span.y - c.from * CH, chunks * CH);
-    const char* record = c.mem + ((size_t)first_of(c, blockIdx.z) * a.H + h) * DELTA_RECORD;
+    const int4 span = span_of(a, of);
+    const int all = min(c.most, (span.y + CH - 1) / CH - c.from), c0 = seg * c.per_seg, chunks = min(c.per_seg, all - c0);
+    const int slices = (a.vdim + 15) / 16;
+    const bool unit = !RESULTS && (int)blockIdx.y >= slices;   // columns of the unit matrix
+    if (chunks <= 0 || (!RESULTS && (c0 + chunks >= all || (unit && seg == 0)))) return;
+    const int slice = unit ? blockIdx.y - slices : blockIdx.y;
+    const int first = span.x + (c.from + c0) * CH, tokens = min(span.y - (c.from + c0) * CH, chunks * CH);
+    const char* record = c.mem + ((size_t)(first_of(c, of) + c0) * a.H + h) * DELTA_RECORD;
     auto rows_of = [&](const void* base, long ld, int at, int i, int width) {   // of chunk i's tokens; behind the last chunk: the last one's
         const int ci = min(i, chunks - 1), n = min(CH, tokens - ci * CH);
         return memory((const char*)base + ((size_t)(first + ci * CH) * ld + at) * ELEM, ((n - 1) * ld + width) * ELEM);
@@ -559,19 +566,26 @@ __global__ __launch_bounds__(512) void k_delta_chunks(DeltaChunks c) {
 
     if (wave < 4) {
         // ================================================================ the chain
-        const int w = wave, col = slice * 16 + x;
-        const bool has_col = col < a.vdim;
+        const int w = wave, col = slice * 16 + x, columns = slices * 16;   // columns: of a start
+        float* start = c.starts + ((size_t)(of * c.segs + seg) * a.H + h) * (32 * DC) * columns;
         float* st = a.state + ((size_t)span.w * a.H + h) * a.dim_kept * a.vdim;
+        // (a portion of one segment has no scouts)
+        const bool from_start = RESULTS && chunks < all, from_slot = RESULTS ? !from_start : !unit && seg == 0, keeps = from_slot && span.z + c.from > 0;
         f4_t S[OWN][2];
-        auto state_at = [&](int j, int half) { return 32 * (w + 4 * j) + 8 * g + 4 * half; };
 #pragma unroll
         for (int j = 0; j < OWN; j++)
 #pragma unroll
             for (int half = 0; half < 2; half++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const int d = state_at(j, half) + r;
-                    S[j][half][r] = span.z + c.from > 0 && has_col && d < a.dim_kept ? st[(size_t)d * a.vdim + col] : 0.f;
+                    const int d = 32 * (w + 4 * j) + 8 * g + 4 * half + r;
+                    float v = unit && d == col ? 1.f : 0.f;
+                    if (d < 32 * DC) {
+                        if (keeps && col < a.vdim && d < a.dim_kept) v = st[(size_t)d * a.vdim + col];
+                        if (from_start) v = start[(size_t)d * columns + col];
+                        if (!RESULTS && seg == 0) start[(size_t)d * columns + col] = v;   // (another workgroup writes the slot later on)
+                    }
+                    S[j][half][r] = v;
                 }
         auto put = [&](u4_t* to, const f4_t& val) {   // [part][64] operands: this tile's half of a lane's eight values
             u2_t parts[3];
@@ -628,7 +642,8 @@ __global__ __launch_bounds__(512) void k_delta_chunks(DeltaChunks c) {
                     for (int t = 0; t < 4; t++) D[t] = mfma6(k[j][t], s, D[t]);
                 }
 #pragma unroll
-                for (int p = 0; p < 3; p++) s_S[(cc * 3 + p) * 64 + lane] = __builtin_bit_cast(u4_t, s[p]);
+                for (int p = 0; p < 3; p++)
+                    if (RESULTS) s_S[(cc * 3 + p) * 64 + lane] = __builtin_bit_cast(u4_t, s[p]);
             }
             if (DC % 4 != 0) asm volatile("s_nop 15" : "+v"(D[0]), "+v"(D[1]), "+v"(D[2]), "+v"(D[3]));   // (they have come over a branch)
             if (SHARES == 4 || w < SHARES)
@@ -734,19 +749,24 @@ __global__ __launch_bounds__(512) void k_delta_chunks(DeltaChunks c) {
                     asm volatile("s_nop 15" : "+v"(S[j][0]), "+v"(S[j][1]));   // (the way round the loop is a branch)
                 }
             }
-            put(s_U + (L::BUFFERS == 2 ? i & 1 : 0) * 384 + (w >> 1) * 192, U);   // (for the results: nobody here waits for it)
+            if (RESULTS) put(s_U + (L::BUFFERS == 2 ? i & 1 : 0) * 384 + (w >> 1) * 192, U);   // (for the results: nobody here waits for it)
             if (L::BUFFERS == 1) __syncthreads();
         }
         __syncthreads();   // U is there
+        if (RESULTS && c0 + chunks < all) return;
+        float* out = RESULTS ? st : unit ? c.trans + ((size_t)(of * c.segs + seg) * a.H + h) * (32 * DC) * (32 * DC) : start + (size_t)a.H * (32 * DC) * columns;
+        const int ld = RESULTS ? a.vdim : unit ? 32 * DC : columns;
 #pragma unroll
         for (int j = 0; j < OWN; j++)
 #pragma unroll
             for (int half = 0; half < 2; half++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const int d = state_at(j, half) + r;
-                    if (has_col && d < a.dim_kept) st[(size_t)d * a.vdim + col] = S[j][half][r];
+                    const int d = 32 * (w + 4 * j) + 8 * g + 4 * half + r;
+                    if (RESULTS ? col < a.vdim && d < a.dim_kept : d < 32 * DC) out[(size_t)d * ld + col] = S[j][half][r];
                 }
+    } else if (!RESULTS && wave < 6) {
+        for (int i = 0; i < (L::BUFFERS == 1 ? 4 : 3) * chunks + 2; i++) __syncthreads();   // (nothing to do but to be counted)
     } else if (wave < 6) {
         // ================================================================ results: lane (x, g) has tokens 16 t + x, columns 4 g .. + 3
         const int t0 = 2 * (wave - 4);   // token tiles t0, t0 + 1
@@ -869,7 +889,7 @@ __global__ __launch_bounds__(512) void k_delta_chunks(DeltaChunks c) {
         const unsigned k_at = 8 * piece < a.dim ? ((unsigned)row * (unsigned)a.k_ld + 8 * piece) * ELEM : NOWHERE, k_step = (128 / ROW) * (unsigned)a.k_ld * ELEM;
         // 16 bytes of a token's 16 values: thread 2 t (+ 1) of token t, in 32 bits 4 t' .. + 3 of tokens t' and 32 + t'
         const int v_col = slice * 16 + (B16 ? 8 * (tid & 1) : 4 * (tid & 3));
-        const unsigned v_ld = (unsigned)a.v_ld * ELEM, v_at = v_col < a.v_cols ? (B16 ? (tid >> 1) * v_ld + 16 * (tid & 1) : (tid >> 2) * v_ld + 16 * (tid & 3)) : NOWHERE;
+        const unsigned v_ld = (unsigned)a.v_ld * ELEM, v_at = v_col < a.v_cols && !unit ? (B16 ? (tid >> 1) * v_ld + 16 * (tid & 1) : (tid >> 2) * v_ld + 16 * (tid & 3)) : NOWHERE;
         const unsigned f_at = tid < 16 ? DELTA_OPS + tid * 16 : tid < 32 ? DELTA_OPS + 2 * CH * 4 + (tid - 16) * 16 : tid == 32 ? DELTA_OPS + 3 * CH * 4 : NOWHERE;
         struct Set {
             u4_t k[ITEMS][W], t[L::STAGED ? 9 : 1], f, v[W];
@@ -884,7 +904,7 @@ __global__ __launch_bounds__(512) void k_delta_chunks(DeltaChunks c) {
                 for (int e = 0; e < W; e++) s.k[n][e] = load16(m, k_at + n * k_step + 16 * e);
         };
         auto fetch_values = [&](Set& s, int i) {
-            const auto m = rows_of(a.v, a.v_ld, h * a.v_cols + slice * 16, i, min(16, a.v_cols - slice * 16));
+            const auto m = rows_of(a.v, a.v_ld, h * a.v_cols + slice * 16, i, unit ? 0 : min(16, a.v_cols - slice * 16));
 #pragma unroll
             for (int e = 0; e < W; e++) s.v[e] = load16(m, v_at + 32 * e * v_ld);
         };
@@ -961,6 +981,79 @@ __global__ __launch_bounds__(512) void k_delta_chunks(DeltaChunks c) {
     }
 }
 
+// The states that a portion's segments start from: start[e + 1] += trans[e] start[e], e = 1 .. (start[1] is complete).  A workgroup =
+// (portion, head, 16 columns), wave w has dim tiles w, w + WAVES; rows of a tile as in k_delta_chunks.  Every step waits for the last one,
+// so the next step's operands travel meanwhile.
+template <int DC>
+constexpr int join_waves() { return DC <= 6 ? 2 * DC : DC; }
+
+template <int DC>
+__global__ __launch_bounds__(64 * join_waves<DC>()) void k_delta_join(DeltaChunks c) {
+    constexpr int WAVES = join_waves<DC>(), TILES = 2 * DC / WAVES;
+    __shared__ u4_t s_S[DC * 192];
+    const Delta& a = c.a;
+    const int h = blockIdx.x, s = blockIdx.z, columns = (a.vdim + 15) & ~15, col0 = blockIdx.y * 16;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), x = lane & 15, g = lane >> 4;
+    const int4 span = span_of(a, s);
+    const int all = min(c.most, (span.y + CH - 1) / CH - c.from), segs = (all + c.per_seg - 1) / c.per_seg;
+    if (segs < 3) return;
+    const size_t step = (size_t)a.H * (32 * DC) * columns, t_step = (size_t)a.H * (32 * DC) * (32 * DC);
+    float* start = c.starts + ((size_t)(s * c.segs) * a.H + h) * (32 * DC) * columns + col0 + x;
+    const float* trans = c.trans + ((size_t)(s * c.segs) * a.H + h) * (32 * DC) * (32 * DC) + 8 * g;
+    int tile[TILES];
+#pragma unroll
+    for (int j = 0; j < TILES; j++) tile[j] = w + WAVES * j;
+    auto at = [&](int j, int r) { return (size_t)(32 * (tile[j] >> 1) + 8 * g + 4 * (tile[j] & 1) + r) * columns; };
+    f4_t S[TILES], next[TILES], m[TILES][DC][2];
+    auto fetch = [&](int e) {   // of the step from start e to start e + 1; behind the last step: its own again
+        const int i = min(e, segs - 2);
+#pragma unroll
+        for (int j = 0; j < TILES; j++) {
+#pragma unroll
+            for (int r = 0; r < 4; r++) next[j][r] = start[(i + 1) * step + at(j, r)];
+            const float* row = trans + i * t_step + (size_t)(32 * (tile[j] >> 1) + 8 * (x >> 2) + 4 * (tile[j] & 1) + (x & 3)) * (32 * DC);
+#pragma unroll
+            for (int cc = 0; cc < DC; cc++)
+#pragma unroll
+                for (int i2 = 0; i2 < 2; i2++) m[j][cc][i2] = *reinterpret_cast<const f4_t*>(row + 32 * cc + 4 * i2);
+        }
+    };
+#pragma unroll
+    for (int j = 0; j < TILES; j++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) S[j][r] = start[step + at(j, r)];
+    fetch(1);
+    for (int e = 1; e + 1 < segs; e++) {
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < TILES; j++) {
+            u2_t parts[3];
+            parts_of_four(S[j], parts);
+#pragma unroll
+            for (int p = 0; p < 3; p++) reinterpret_cast<u2_t*>(s_S + ((tile[j] >> 1) * 3 + p) * 64 + lane)[tile[j] & 1] = parts[p];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < TILES; j++) {
+            f4_t sum[2] = {next[j], {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+            for (int cc = 0; cc < DC; cc++) {
+                b8_t mp[3], sp[3];
+                parts_of_eight(m[j][cc][0], m[j][cc][1], mp);
+#pragma unroll
+                for (int p = 0; p < 3; p++) sp[p] = __builtin_bit_cast(b8_t, s_S[(cc * 3 + p) * 64 + lane]);
+                sum[cc & 1] = mfma6(mp, sp, sum[cc & 1]);
+            }
+            S[j] = sum[0] + sum[1];
+        }
+        fetch(e + 1);
+#pragma unroll
+        for (int j = 0; j < TILES; j++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) start[(e + 1) * step + at(j, r)] = S[j][r];
+    }
+}
+
 // Rows of queries and keys whose dims or addresses the chunk kernels' loads do not fit: dims padded to a multiple of 8 with zeros.
 // (The same for values.)
 template <typename E>
@@ -972,22 +1065,37 @@ __global__ __launch_bounds__(256) void k_delta_rows(E* __restrict__ dst, const E
     }
 }
 
+template <typename F>
+static void more_lds(F* kernel, int bytes) {
+    HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+}
 template <int DC, bool B16>
 static void launch_chunks_of(const DeltaChunks& c) {
     const Delta& a = c.a;
     constexpr int prep = prepare_lds<DC, B16>(), walk = Walk<DC, B16>::LDS;
     static bool enabled = false;
     if (!enabled) {
-        HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(&k_delta_prepare<DC, B16>), hipFuncAttributeMaxDynamicSharedMemorySize, prep));
-        HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(&k_delta_chunks<DC, B16>), hipFuncAttributeMaxDynamicSharedMemorySize, walk));
+        more_lds(&k_delta_prepare<DC, B16>, prep);
+        more_lds(&k_delta_chunks<DC, B16, true>, walk);
+        more_lds(&k_delta_chunks<DC, B16, false>, walk);
         enabled = true;
     }
+    const int slices = cdiv(a.vdim, 16), launches = c.segs == 1 ? 2 : 4;
+    const double bytes = c.bytes / launches, flops = c.flops / launches;
     {
-        ProfScope ps(PC_DELTA, c.bytes / 2, c.flops / 2);
+        ProfScope ps(PC_DELTA, bytes, flops);
         NVLLM_LAUNCH((k_delta_prepare<DC, B16>), dim3(a.H, c.most, a.n_spans), dim3(256), prep, c);
     }
-    ProfScope ps(PC_DELTA, c.bytes / 2, c.flops / 2);
-    NVLLM_LAUNCH((k_delta_chunks<DC, B16>), dim3(a.H, cdiv(a.vdim, 16), a.n_spans), dim3(512), walk, c);
+    if (c.segs > 1) {
+        ProfScope ps(PC_DELTA, bytes, flops);
+        NVLLM_LAUNCH((k_delta_chunks<DC, B16, false>), dim3(a.H, slices + 2 * DC, a.n_spans * c.segs), dim3(512), walk, c);
+    }
+    if (c.segs > 1) {
+        ProfScope ps(PC_DELTA, bytes, flops);
+        NVLLM_LAUNCH((k_delta_join<DC>), dim3(a.H, slices, a.n_spans), dim3(64 * join_waves<DC>()), 0, c);
+    }
+    ProfScope ps(PC_DELTA, bytes, flops);
+    NVLLM_LAUNCH((k_delta_chunks<DC, B16, true>), dim3(a.H, slices, a.n_spans * c.segs), dim3(512), walk, c);
 }
 template <bool B16>
 static void launch_chunks(const DeltaChunks& c) {
@@ -1018,21 +1126,50 @@ static int delta_spans(std::vector<int4>& spans, const int* seq_ids, const int* 
     return std::adjacent_find(ids.begin(), ids.end()) == ids.end() ? 0 : NVLLM_BAD_INDEX;
 }
 
-// Where a batch's portions go: the first n_chunked by chunks, the others token by token.
-constexpr int CHUNK_MIN = 16;                          // tokens of a portion that goes by chunks
-constexpr size_t CHUNK_MEMORY = (size_t)192 << 20;     // of the chunks' records at a time
+constexpr size_t CHUNK_MEMORY = (size_t)192 << 20;   // of the chunks' records at a time
+
+// Tokens from which a portion goes by chunks.  A token of a portion costs 1.2 us on the way token by token (128 dims), 4 us where states by
+// the hundred fill the chip; a chunk costs 14 us (19 us in 32 bits) whatever its tokens, and 5 us (8 us) more for every 256 workgroups
+// behind the first.  Measured, token by token and by chunks, heads of 128 x 128 in bf16: 32 heads, 8 tokens 15.4 and 14.1 us ... 20.2 and
+// 14.2 for 12; eight sequences (2,048 workgroups), 16 tokens: 30 and 46, 24: 42 and 46, 32: 53 and 47; 32 sequences, 32 tokens: 139 and 162,
+// 48: 204 and 170.
+constexpr int CHUNK_LEAST = 8;
+static int chunk_min(const Delta& a, const std::vector<int4>& spans, bool b16) {
+    double wgs = 0;
+    for (const int4& s : spans) wgs += s.y >= CHUNK_LEAST ? (double)a.H * cdiv(a.vdim, 16) : 0.0;
+    return (int)((b16 ? 1.0 : 1.5) * CHUNK_LEAST * sqrt(std::max(1.0, wgs / 256)));
+}
+
+// Segments of the portions' chunks, walked side by side, where heads and columns alone leave most of the chip empty.  They cost another walk
+// for what a segment does to a state (its scouts), of which as many run at a time as there are CUs, and a join in which one start waits for
+// the other; n segments of m chunks take about m / n + DC n / 2.5 of a chunk's time, least at sqrt(2.5 m / DC).  Measured, in one segment and
+// in this many: 8,192 tokens, one head of 128 x 128: 212 us, 87 in 8; four: 212, 109 in 5; eight: 218, 154 in 3 (166 in 4, which no longer fit
+// side by side); one of 64 x 64: 201, 69 in 12; 4,096 tokens, two of 256 x 256: 157, 119 in 4; 1,024 tokens, one of 128 x 128: 38, 41 in 3.
+static void delta_segments(DeltaChunks& c, int DC, int most) {
+    const Delta& a = c.a;
+    const long walks = (long)a.H * cdiv(a.vdim, 16) * a.n_spans, unit = (long)a.H * 2 * DC * a.n_spans, cus = rt().num_cus;
+    c.segs = 1;
+    c.per_seg = most;
+    if (most < 6 * DC || walks + unit > cus) return;
+    const long fit = std::min(2 + (cus - walks) / (walks + unit), cus / walks), best = (long)sqrt(2.5 * most / DC);
+    const int segs = (int)std::min(fit, best);
+    if (segs < 3) return;
+    c.per_seg = cdiv(most, segs);
+    c.segs = cdiv(most, c.per_seg);
+}
 
 static int gated_delta(Delta& a, const int* seq_ids, const int* pos, int T, int n_slots, int elem) {
     std::vector<int4> spans;
     if (const int e = delta_spans(spans, seq_ids, pos, T, n_slots)) return e;
     if ((double)cdiv(a.vdim, STEP_COLS) * a.H * (double)spans.size() > 2e9) return NVLLM_BAD_SIZE;
     const bool b16 = elem == 2;
-    std::stable_sort(spans.begin(), spans.end(), [](const int4& l, const int4& r) { return (l.y >= CHUNK_MIN) > (r.y >= CHUNK_MIN); });
+    const int least = chunk_min(a, spans, b16);   // portions that go by chunks come first
+    std::stable_sort(spans.begin(), spans.end(), [&](const int4& l, const int4& r) { return (l.y >= least) > (r.y >= least); });
     int n_chunked = 0, longest = 0;
     long tokens = 0;
     double states[2] = {0, 0};
     for (const int4& s : spans) {
-        const bool ch = s.y >= CHUNK_MIN;
+        const bool ch = s.y >= least;
         states[ch] += (s.z > 0 ? 8.0 : 4.0) * a.H * a.dim * (double)a.vdim;
         if (!ch) continue;
         n_chunked++;
@@ -1086,12 +1223,15 @@ static int gated_delta(Delta& a, const int* seq_ids, const int* pos, int T, int 
         c.out_four = a.vdim % 4 == 0 && (size_t)a.out % (4 * elem) == 0;
         size_t n_records = 0;
         for (int i = 0; i < n_chunked; i++) n_records = std::max(n_records, (size_t)first[i] + std::min(most, cdiv(spans[i].y, CH)));
+        const int steps = cdiv(a.dim, 32), DC = steps <= 4 ? steps : steps <= 6 ? 6 : 8;
+        delta_segments(c, DC, most);
+        const size_t columns = (size_t)((a.vdim + 15) & ~15), places = c.segs > 1 ? (size_t)n_chunked * c.segs * a.H * (32 * DC) : 0;
         const int per16 = 16 / elem, dim_ld = (a.dim + 7) & ~7, vdim_ld = (a.vdim + 7) & ~7;
         const bool fits = a.dim % 8 == 0 && a.q_ld % per16 == 0 && a.k_ld % per16 == 0 && ((size_t)a.q | (size_t)a.k) % 16 == 0;
         const bool v_fits = a.vdim % per16 == 0 && a.v_ld % per16 == 0 && (size_t)a.v % 16 == 0;
         auto room = [&](bool needed, int heads, int ld) { return needed ? ((size_t)T * heads * ld * elem + 255) & ~(size_t)255 : 0; };
         const size_t qk_room = room(!fits, a.Q, dim_ld), v_room = room(!v_fits, a.H, vdim_ld);
-        char* mem = (char*)ws_get(WS_DELTA, 2 * qk_room + v_room + n_records * a.H * DELTA_RECORD);
+        char* mem = (char*)ws_get(WS_DELTA, 2 * qk_room + v_room + n_records * a.H * DELTA_RECORD + places * (columns + 32 * DC) * sizeof(float));
         auto pack = [&](const void*& src, long& ld, int heads, int dim, int wide) {
             if (b16) NVLLM_LAUNCH((k_delta_rows<unsigned short>), dim3(T), dim3(256), 0, (unsigned short*)mem, (const unsigned short*)src, heads, dim, wide, ld);
             else NVLLM_LAUNCH((k_delta_rows<float>), dim3(T), dim3(256), 0, (float*)mem, (const float*)src, heads, dim, wide, ld);
@@ -1112,6 +1252,8 @@ static int gated_delta(Delta& a, const int* seq_ids, const int* pos, int T, int 
             c.a.v_cols = vdim_ld;
         }
         c.mem = mem;
+        c.starts = (float*)(mem + n_records * a.H * DELTA_RECORD);
+        c.trans = c.starts + places * columns;
         // the algorithm's bytes and flops, split over the launches
         const int rounds = cdiv(longest, most);
         c.bytes = (states[1] + (double)tokens * token_bytes) / rounds;

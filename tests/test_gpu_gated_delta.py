@@ -122,6 +122,47 @@ def test_a_long_portion(hip, elem):
 
 
 @BOTH
+@pytest.mark.parametrize("n", [6, 7, 8, 9, 11, 12, 13, 22, 23, 33, 34])
+def test_short_portions(hip, elem, n):
+    """About the lengths at which chunks take over, which rise with the batch."""
+    check(hip, elem, [(1, 0, n), (0, 60, n + 1)], 2, 2, 64, 48)
+    check(hip, elem, [(i, 3 * i, n + i % 2) for i in range(8)], 16, 32, 32, 128)
+
+
+# few heads and many tokens: such portions are walked in segments side by side; heads of every number of 32 dims, columns off every width
+LONG = [(1, 2, 32, 20, 900), (1, 1, 64, 64, 1500), (1, 3, 80, 16, 1300), (2, 2, 128, 40, 1700), (1, 1, 192, 24, 2400), (1, 1, 256, 33, 3200)]
+
+
+@BOTH
+@pytest.mark.parametrize("heads", LONG, ids=str)
+def test_long_portions_of_few_heads(hip, elem, heads):
+    """Beside portions of a chunk, of half the length and of a token."""
+    *heads, n = heads
+    check(hip, elem, [(2, 0, n)], *heads)
+    check(hip, elem, [(2, 9, n), (0, 70, 50), (1, 5, 1), (5, 0, n // 2 + 3), (3, 0, 65)], *heads, seed=1)
+
+
+@BOTH
+def test_gates_of_long_portions(hip, elem):
+    """Heads that hold what they read over the whole portion, that lose all of it in the middle, that never write; a slot of rubbish."""
+    def gates(q, k, v, g, beta, state):
+        g[:, 0], beta[:, 0] = 0.0, 0.01
+        g[700, 1] = -np.inf
+        beta[:, 2] = 0.0
+        g[:, 2] = -1e-4
+        g[:, 3] = -60.0
+        state[1] = np.nan
+    check(hip, elem, [(0, 9, 1600), (1, 0, 1100)], 2, 4, 64, 32, edit=gates)
+
+
+@pytest.mark.parametrize("heads", [(16, 16, 32, 16, 40000), (256, 256, 32, 16, 2400)], ids=str)
+def test_more_chunks_than_are_prepared_at_a_time(hip, heads):
+    """With segments (16 heads) and without; the state goes on from one round of chunks to the next."""
+    *heads, n = heads
+    check(hip, O.BF16, [(0, 3, n), (1, 0, 100)], *heads)
+
+
+@BOTH
 def test_many_sequences(hip, elem):
     """More portions than travel with a launch's arguments, slots in no order."""
     order = np.random.Generator(np.random.PCG64(5)).permutation(90)
@@ -210,6 +251,15 @@ def test_portions_one_after_the_other(hip, elem):
 def test_the_same_call_twice_gives_the_same_bits(hip, elem):
     data = O.inputs(11, 700, 4, 4, 128, 128, elem, 3)
     spans = [(2, 0, 500), (0, 70, 130), (1, 3, 70)]
+    a, b = (call(hip, data, spans, elem, 0.1, 1e-6) for _ in range(2))
+    np.testing.assert_array_equal(a[0], b[0])
+    np.testing.assert_array_equal(a[1], b[1])
+
+
+@BOTH
+def test_a_long_portion_twice_gives_the_same_bits(hip, elem):
+    data = O.inputs(12, 1700, 1, 2, 128, 128, elem, 3)
+    spans = [(2, 0, 1600), (0, 70, 100)]
     a, b = (call(hip, data, spans, elem, 0.1, 1e-6) for _ in range(2))
     np.testing.assert_array_equal(a[0], b[0])
     np.testing.assert_array_equal(a[1], b[1])
