@@ -263,7 +263,7 @@ constexpr unsigned NOWHERE = 0x80000000u;
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t memory(const void* base, long bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)bytes, 0x00020000);
 }
-__device__ __forceinline__ u4_t load16(__amdgpu_buffer_rsrc_t m, unsigned at) { return __builtin_bit_cast(u4_t, __builtin_amdgcn_raw_buffer_load_b128(m, (int)at, 0, 0)); }
+__device__ __forceinline__ u4_t load16(__amdgpu_buffer_rsrc_t m, unsigned at, int base = 0) { return __builtin_bit_cast(u4_t, __builtin_amdgcn_raw_buffer_load_b128(m, (int)at, base, 0)); }
 __device__ __forceinline__ float load4(__amdgpu_buffer_rsrc_t m, unsigned at) { return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(m, (int)at, 0, 0)); }
 
 // A token's row of queries or keys as operands: lane (x, g) has dims 32 cc + 8 g .. + 7 of the tile's row x.
@@ -521,21 +521,22 @@ __global__ __launch_bounds__(256) void k_delta_prepare(DeltaChunks c) {
 template <int DC, bool B16>
 struct Walk {
     static constexpr int PARTS = B16 ? 1 : 3;
-    static constexpr int STATE = DC * DELTA_TILE, SHARES = 16 * 1024, EX = 2 * DELTA_TILE, KEYS = DC * PARTS * 4096, OPS = 7 * DELTA_TILE, VALUES = 4096, FACTORS = 1024;
+    static constexpr int STATE = DC * DELTA_TILE, SHARES = (DC < 4 ? DC : 4) * 4096, EX = 2 * DELTA_TILE, KEYS = DC * PARTS * 4096, OPS = 7 * DELTA_TILE, VALUES = 4096, FACTORS = 1024;
     static constexpr int REST = STATE + SHARES + 3 * EX + VALUES + FACTORS, MOST = 160 * 1024;
     static constexpr bool STAGED = REST + KEYS + OPS <= MOST;                          // T' goes through LDS
     static constexpr int BUFFERS = REST + EX + 2 * KEYS + OPS <= MOST ? 2 : 1;         // of keys and of U
     static constexpr int LDS = REST + (BUFFERS - 1) * EX + BUFFERS * KEYS + (STAGED ? OPS : 0);
+    static constexpr bool PAIR = B16 && 2 * LDS <= MOST;   // two workgroups on a CU
 };
 
 template <int DC, bool B16, bool RESULTS>
-__global__ __launch_bounds__(512) void k_delta_chunks(DeltaChunks c) {
+__global__ __launch_bounds__(512, (Walk<DC, B16>::PAIR ? 4 : 2)) void k_delta_chunks(DeltaChunks c) {
     typedef Walk<DC, B16> L;
     constexpr int PARTS = L::PARTS, OWN = (DC + 3) / 4, SHARES = DC < 4 ? DC : 4, ELEM = B16 ? 2 : 4;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds_d[];
     u4_t* s_S = reinterpret_cast<u4_t*>(lds_d);            // [DC][part][64] the state as operand
     f4_t* s_D = reinterpret_cast<f4_t*>(s_S + DC * 192);   // [wave][token tile][64] shares of S^T k
-    u4_t* s_X = reinterpret_cast<u4_t*>(s_D + 16 * 64);    // [32 tokens][part][64]
+    u4_t* s_X = reinterpret_cast<u4_t*>(s_D + SHARES * 256);    // [32 tokens][part][64]
     u4_t* s_U = s_X + 6 * 64;                              // [buffer]
     u4_t* s_V = s_U + L::BUFFERS * 6 * 64;                 // U as the state takes it
     u4_t* s_v = s_V + 6 * 64;                              // [token][16] values
@@ -779,7 +780,7 @@ __global__ __launch_bounds__(512) void k_delta_chunks(DeltaChunks c) {
             float fb[2];
             b8_t po[2][2][3];
         };
-        constexpr int SETS = sizeof(Set) / 4 <= 84 ? 2 : 1;   // (chunks in flight: what fits the registers)
+        constexpr int SETS = !L::PAIR && sizeof(Set) / 4 <= 84 ? 2 : 1;   // (chunks in flight: what fits the registers)
         Set set[SETS];
         auto fetch_queries = [&](Set& s, int i) {
             const auto m = record_of(i);
@@ -798,18 +799,24 @@ __global__ __launch_bounds__(512) void k_delta_chunks(DeltaChunks c) {
                 for (int p = 0; p < 2; p++)
 #pragma unroll
                     for (int j = 0; j < 3; j++)
-                        s.po[t][p][j] = __builtin_bit_cast(b8_t, load16(m, p == 0 || t0 > 0 ? (6 + op_tile(t0 + t, p)) * DELTA_TILE + j * DELTA_PART + lane * 16 : NOWHERE));
+                        s.po[t][p][j] = __builtin_bit_cast(b8_t, load16(m, p == 0 || t0 > 0 ? lane * 16 : NOWHERE, (6 + op_tile(t0 + t, p)) * DELTA_TILE + j * DELTA_PART));
         };
         f4_t o[2];
         auto finish = [&](const Set& s, int i) {   // chunk i's results: U has come
             b8_t e[2][3];
             const u4_t* U = s_U + (L::BUFFERS == 2 ? i & 1 : 0) * 384;
             get(U, e[0]);
+            f4_t first[2];
+            if (L::PAIR) {   // (one after the other: registers)
+#pragma unroll
+                for (int t = 0; t < 2; t++) first[t] = mfma6(e[0], s.po[t][0], o[t]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
             get(U + 192, e[1]);
             const auto m = rows_of(a.out, (long)a.H * a.vdim, h * a.vdim + slice * 16, i, min(16, a.vdim - slice * 16));
 #pragma unroll
             for (int t = 0; t < 2; t++) {
-                const f4_t y = mfma6(e[0], s.po[t][0], o[t]) + mfma6(e[1], s.po[t][1], zero);
+                const f4_t y = L::PAIR ? mfma6(e[1], s.po[t][1], first[t]) : mfma6(e[0], s.po[t][0], o[t]) + mfma6(e[1], s.po[t][1], zero);
                 const unsigned at = o_row + t * o_tile;
                 if (c.out_four) {
                     if (B16) __builtin_amdgcn_raw_buffer_store_b64(u2_t{two_b16(y[0], y[1]), two_b16(y[2], y[3])}, m, (int)(has_out[0] ? at : NOWHERE), 0, 0);
@@ -894,7 +901,7 @@ __global__ __launch_bounds__(512) void k_delta_chunks(DeltaChunks c) {
         struct Set {
             u4_t k[ITEMS][W], t[L::STAGED ? 9 : 1], f, v[W];
         };
-        constexpr int SETS = sizeof(Set) / 4 <= 88 ? 2 : 1;   // (chunks in flight: what fits the registers)
+        constexpr int SETS = !L::PAIR && sizeof(Set) / 4 <= 88 ? 2 : 1;   // (chunks in flight: what fits the registers)
         Set set[SETS];
         auto fetch_keys = [&](Set& s, int i) {
             const auto m = rows_of(a.k, a.k_ld, hq * a.dim, i, a.dim);
