@@ -35,8 +35,9 @@ struct DeltaChunks {
     const int* first;           // [n_spans] the launch's first chunk of each span; null: the ones here
     int first_here[DELTA_SPANS];
     int from, most;             // chunks [from, from + most) of every span
+    int step_waves;             // of portions behind the first n_spans, which go token by token beside the first chunks
     int segs, per_seg;          // segments of a portion's chunks of the launch at most, chunks of one
-    float* starts;              // [span][segs][H][dims][columns] states that segments start from, both padded (see k_delta_walk) ...
+    float* starts;              // [span][segs][H][dims][columns] states that segments start from, both padded ...
     float* trans;               // [span][segs][H][dims][dims] ... and what becomes of a state over a segment
     bool out_four;              // out can be stored four elements at a time
     double bytes, flops;        // kernel timing

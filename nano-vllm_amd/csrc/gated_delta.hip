@@ -85,16 +85,15 @@ __device__ __forceinline__ float sum_over_rows(float x) {
 constexpr int STEP_COLS = 32;   // of a wave
 
 template <bool B16, int NR, bool VEC>
-__global__ __launch_bounds__(64) void k_delta_step(Delta a) {
+__device__ __forceinline__ void delta_step(const Delta& a, int idx, int lane) {   // idx = (portion, head, slice) of the wave
     constexpr int R4 = NR / 4;
     typedef Four<B16, VEC> F;
     const int slices = (a.vdim + STEP_COLS - 1) / STEP_COLS;
-    int idx = blockIdx.x;
     const int slice = idx % slices;
     idx /= slices;
     const int h = idx % a.H;
     const int4 span = (a.spans ? a.spans : a.here)[idx / a.H];
-    const int lane = threadIdx.x, col = slice * STEP_COLS + (lane & 7) * 4, row0 = (lane >> 3) * NR, hq = h / (a.H / a.Q);
+    const int col = slice * STEP_COLS + (lane & 7) * 4, row0 = (lane >> 3) * NR, hq = h / (a.H / a.Q);
     const int cols = a.vdim - col, rows = a.dim - row0;   // that this lane has at most
     float* st = a.state + ((size_t)span.w * a.H + h) * a.dim * a.vdim;
     f4_t S[NR];
@@ -173,6 +172,9 @@ __global__ __launch_bounds__(64) void k_delta_step(Delta a) {
     for (int r = 0; r < NR; r++)
         if (r < rows) store_four<false, VEC>(st, (size_t)(row0 + r) * a.vdim + col, S[r], cols);
 }
+
+template <bool B16, int NR, bool VEC>
+__global__ __launch_bounds__(64) void k_delta_step(Delta a) { delta_step<B16, NR, VEC>(a, blockIdx.x, threadIdx.x); }
 
 template <bool B16, bool VEC>
 static void launch_step(const Delta& a) {
@@ -340,7 +342,7 @@ constexpr int prepare_keys() { return std::max(4 * DC * (B16 ? 1 : 3) * 1024, CH
 template <int DC, bool B16>
 constexpr int prepare_lds() { return prepare_keys<DC, B16>() + CH * LD * 4 + CH * (8 + 4 + 4); }
 
-template <int DC, bool B16>
+template <int DC, bool B16, bool STEPS>
 __global__ __launch_bounds__(256) void k_delta_prepare(DeltaChunks c) {
     constexpr int PARTS = B16 ? 1 : 3;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds_d[];
@@ -351,6 +353,11 @@ __global__ __launch_bounds__(256) void k_delta_prepare(DeltaChunks c) {
     float* s_r = reinterpret_cast<float*>(s_G + CH);                       // what norms a key
     float* s_b = s_r + CH;
     const Delta& a = c.a;
+    if (STEPS && (int)blockIdx.z >= a.n_spans) {   // portions that go token by token, behind the others
+        const int wave = (((blockIdx.z - a.n_spans) * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        if (wave < c.step_waves) delta_step<B16, 4 * DC, true>(a, a.n_spans * a.H * ((a.vdim + STEP_COLS - 1) / STEP_COLS) + wave, threadIdx.x & 63);
+        return;
+    }
     const int h = blockIdx.x, hq = h / (a.H / a.Q);
     const ChunkAt at = chunk_at(c, blockIdx.z, h, blockIdx.y);
     if (at.n <= 0) return;
@@ -1082,7 +1089,8 @@ static void launch_chunks_of(const DeltaChunks& c) {
     constexpr int prep = prepare_lds<DC, B16>(), walk = Walk<DC, B16>::LDS;
     static bool enabled = false;
     if (!enabled) {
-        more_lds(&k_delta_prepare<DC, B16>, prep);
+        more_lds(&k_delta_prepare<DC, B16, false>, prep);
+        more_lds(&k_delta_prepare<DC, B16, true>, prep);
         more_lds(&k_delta_chunks<DC, B16, true>, walk);
         more_lds(&k_delta_chunks<DC, B16, false>, walk);
         enabled = true;
@@ -1091,7 +1099,8 @@ static void launch_chunks_of(const DeltaChunks& c) {
     const double bytes = c.bytes / launches, flops = c.flops / launches;
     {
         ProfScope ps(PC_DELTA, bytes, flops);
-        NVLLM_LAUNCH((k_delta_prepare<DC, B16>), dim3(a.H, c.most, a.n_spans), dim3(256), prep, c);
+        if (c.step_waves > 0) NVLLM_LAUNCH((k_delta_prepare<DC, B16, true>), dim3(a.H, c.most, a.n_spans + cdiv(c.step_waves, 4 * a.H * c.most)), dim3(256), prep, c);
+        else NVLLM_LAUNCH((k_delta_prepare<DC, B16, false>), dim3(a.H, c.most, a.n_spans), dim3(256), prep, c);
     }
     if (c.segs > 1) {
         ProfScope ps(PC_DELTA, bytes, flops);
@@ -1216,6 +1225,10 @@ static int gated_delta(Delta& a, const int* seq_ids, const int* pos, int T, int 
         d_spans = (const int4*)dev;
         d_first = dev + 4 * spans.size();
     }
+    const size_t four = 4 * (size_t)elem;
+    const bool vec = a.dim % 4 == 0 && a.vdim % 4 == 0 && a.q_ld % 4 == 0 && a.k_ld % 4 == 0 && a.v_ld % 4 == 0 && (size_t)a.q % four == 0 && (size_t)a.k % four == 0 &&
+                     (size_t)a.v % four == 0 && (size_t)a.out % four == 0 && (size_t)a.state % 16 == 0;
+    a.n_spans = (int)spans.size() - n_chunked;
     const double token_bytes = elem * (2.0 * a.Q * a.dim + 2.0 * a.H * a.vdim) + 8.0 * a.H, token_flops = 6.0 * a.H * a.dim * (double)a.vdim;
     if (n_chunked > 0) {
         DeltaChunks c{};
@@ -1224,7 +1237,7 @@ static int gated_delta(Delta& a, const int* seq_ids, const int* pos, int T, int 
         c.a.spans = d_spans;
         c.first = d_first;
         if (!d_spans) {
-            std::copy(spans.begin(), spans.begin() + n_chunked, c.a.here);
+            std::copy(spans.begin(), spans.end(), c.a.here);
             std::copy(first.begin(), first.begin() + n_chunked, c.first_here);
         }
         c.out_four = a.vdim % 4 == 0 && (size_t)a.out % (4 * elem) == 0;
@@ -1265,19 +1278,25 @@ static int gated_delta(Delta& a, const int* seq_ids, const int* pos, int T, int 
         const int rounds = cdiv(longest, most);
         c.bytes = (states[1] + (double)tokens * token_bytes) / rounds;
         c.flops = (double)tokens * token_flops / rounds;
+        // The others' steps go with the first chunks' launch where rows are aligned for both, unless there are chunks for several turns on
+        // every CU, which then run fewer at a time (in 16 bits; in 32 they take as many registers as the steps).  Apart and together:
+        // three portions of 512 tokens and eleven of one, 32 heads of 64 x 64: 40.0 us, 36.8; one of 512 and 64, 128 x 128: 94, 84 (in
+        // 32 bits 111, 98); four of 1,024 and 64: 226, 230 (362, 347).
+        const long waves = (long)cdiv(a.vdim, STEP_COLS) * a.H * ((long)spans.size() - n_chunked);
+        if (fits && v_fits && vec && (!b16 || n_records * a.H <= 4 * (size_t)rt().num_cus) && n_chunked + waves / (4L * a.H * most) < 65535) {
+            c.step_waves = (int)waves;
+            a.n_spans = 0;
+        }
         for (c.from = 0; c.from < longest; c.from += most) {
             c.most = std::min(most, longest - c.from);
             if (b16) launch_chunks<true>(c);
             else launch_chunks<false>(c);
+            c.step_waves = 0;
         }
     }
-    a.n_spans = (int)spans.size() - n_chunked;
     if (a.n_spans == 0) return 0;
     a.spans = d_spans ? d_spans + n_chunked : nullptr;
     if (!d_spans) std::copy(spans.begin() + n_chunked, spans.end(), a.here);
-    const size_t four = 4 * (size_t)elem;
-    const bool vec = a.dim % 4 == 0 && a.vdim % 4 == 0 && a.q_ld % 4 == 0 && a.k_ld % 4 == 0 && a.v_ld % 4 == 0 && (size_t)a.q % four == 0 && (size_t)a.k % four == 0 &&
-                     (size_t)a.v % four == 0 && (size_t)a.out % four == 0 && (size_t)a.state % 16 == 0;
     ProfScope ps(PC_DELTA_TOK, states[0] + (double)(T - tokens) * token_bytes, (double)(T - tokens) * token_flops);
     if (b16 && vec) launch_step<true, true>(a);
     else if (b16) launch_step<true, false>(a);

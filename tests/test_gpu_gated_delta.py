@@ -265,6 +265,43 @@ def test_a_long_portion_twice_gives_the_same_bits(hip, elem):
     np.testing.assert_array_equal(a[1], b[1])
 
 
+@BOTH
+@pytest.mark.parametrize("heads", [(2, 2, 32, 40), (2, 4, 64, 64)], ids=str)
+def test_portions_beside_single_tokens(hip, elem, heads):
+    """Single tokens of a batch with portions go with the portions' first launch; here more sequences than travel with its arguments, and fewer."""
+    for many in (130, 60):
+        order = np.random.Generator(np.random.PCG64(many)).permutation(many + 5)
+        check(hip, elem, [(int(s), i % 4, 1 if i % 5 else 20 + 3 * i) for i, s in enumerate(order[:many])], *heads, slots=many + 5)
+
+
+@BOTH
+def test_samples_and_beams_of_one_prompt(hip, elem):
+    """As a program uses the two together: a prompt, its state to the samples' slots, then steps before each of which every sample goes on from
+    the state of a chosen one."""
+    Q, H, dim, vdim, slots, n, steps = 2, 4, 64, 48, 7, 5, 12
+    scale, size = np.float32(0.125), 4 * H * dim * vdim
+    r = np.random.Generator(np.random.PCG64(21))
+    *data, state = O.inputs(22, 90, Q, H, dim, vdim, elem, slots)
+    got, st = call(hip, (*data, state), [(6, 0, 90)], elem, scale, 1e-6)
+    want, exact = O.forward(*data, state, [(6, 0, 90)], scale, 1e-6)
+    most = O.limit(90 + steps, dim)
+    assert O.off(got, want, elem) <= most
+    to, frm, at = [3, 0, 5, 1, 2], [6] * n, 90
+    for step in range(steps):
+        p = hip.to_device(st)
+        assert hip.nvllm_copy_states(p, size, 1, slots, capi.ints(frm), capi.ints(to), n) == 0
+        st = hip.to_host(p, st.shape, np.float32)
+        hip.free(p)
+        exact[to] = exact[frm]
+        *data, _ = O.inputs(100 + step, n, Q, H, dim, vdim, elem, 1)
+        spans = [(s, at, 1) for s in to]
+        got, st = call(hip, (*data, st), spans, elem, scale, 1e-6)
+        want, exact = O.forward(*data, exact, spans, scale, 1e-6)
+        worst = O.off(got, want, elem), O.off(st[to], exact[to])
+        assert max(worst) <= most, (step, worst)
+        frm, at = [to[i] for i in r.integers(0, n, n)], at + 1
+
+
 def test_a_captured_stream_is_refused(hip):
     """The host arrays are read at the call, so a replay would not see them; nothing is enqueued."""
     rtl = C.CDLL("libamdhip64.so")
