@@ -695,25 +695,31 @@ __global__ __launch_bounds__(512, (Walk<DC, B16>::PAIR ? 4 : 2)) void k_delta_ch
             b8_t e[2][3];
             get(s_X, e[0]);
             get(s_X + 192, e[1]);
-            // keys as columns (16 lanes bring 4 tokens x 16 dims, lane x receives dim x of the four), and the next chunk's
+            // Keys as columns (16 lanes bring 4 tokens x 16 dims, lane x receives dim x of the four), and the next chunk's.  Where they are
+            // many and of one part they are asked for behind U's products, which need not wait for them (LDS gives 128 bytes a clock to
+            // all waves: 16 heads of 128 x 128 over 8,192 tokens 230 -> 222 us; in 32 bits and for 64 dims it costs 1 %).
+            constexpr bool LATE = B16 && DC % 4 == 0;
             b8_t kt[OWN][2][2][PARTS];
+            auto read_columns = [&] {
 #pragma unroll
-            for (int j = 0; j < OWN; j++) {
-                const int cc = w + 4 * j;
-                if (DC % 4 != 0 && cc >= DC) break;
+                for (int j = 0; j < OWN; j++) {
+                    const int cc = w + 4 * j;
+                    if (DC % 4 != 0 && cc >= DC) break;
 #pragma unroll
-                for (int half = 0; half < 2; half++)
+                    for (int half = 0; half < 2; half++)
 #pragma unroll
-                    for (int p = 0; p < 2; p++)
+                        for (int p = 0; p < 2; p++)
 #pragma unroll
-                        for (int part = 0; part < PARTS; part++) {
-                            const u2_t* at = reinterpret_cast<const u2_t*>(keys_of(i) + ((cc * PARTS + part) * CH + 32 * p + 4 * g + (x >> 2)) * 4 + (x & 3)) + half;
-                            const u2_t lo = __builtin_bit_cast(u2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)at));
-                            const u2_t hi = __builtin_bit_cast(u2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at + 16 * 8)));
-                            kt[j][half][p][part] = __builtin_bit_cast(b8_t, u4_t{lo[0], lo[1], hi[0], hi[1]});
-                        }
-                if (L::BUFFERS == 2) read_keys(i + 1, j);
-            }
+                            for (int part = 0; part < PARTS; part++) {
+                                const u2_t* at = reinterpret_cast<const u2_t*>(keys_of(i) + ((cc * PARTS + part) * CH + 32 * p + 4 * g + (x >> 2)) * 4 + (x & 3)) + half;
+                                const u2_t lo = __builtin_bit_cast(u2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)at));
+                                const u2_t hi = __builtin_bit_cast(u2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at + 16 * 8)));
+                                kt[j][half][p][part] = __builtin_bit_cast(b8_t, u4_t{lo[0], lo[1], hi[0], hi[1]});
+                            }
+                    if (!LATE && L::BUFFERS == 2) read_keys(i + 1, j);
+                }
+            };
+            if (!LATE) read_columns();
             __builtin_amdgcn_sched_barrier(0);
             f4_t U0 = mfma(to[0][1], e[0][1], zero), U1 = mfma(to[0][1], e[0][0], zero), U2 = mfma(to[1][1], e[1][1], zero), U3 = mfma(to[1][1], e[1][0], zero);
             U0 = mfma(to[0][2], e[0][0], U0);
@@ -724,6 +730,11 @@ __global__ __launch_bounds__(512, (Walk<DC, B16>::PAIR ? 4 : 2)) void k_delta_ch
             U1 = mfma(to[0][0], e[0][0], U1);
             U2 = mfma(to[1][0], e[1][2], U2);
             U3 = mfma(to[1][0], e[1][0], U3);
+            if (LATE) {
+                __builtin_amdgcn_sched_barrier(0);
+                read_columns();
+                __builtin_amdgcn_sched_barrier(0);
+            }
             const f4_t U = (U0 + U2) + (U1 + U3);
             put(s_V + (w >> 1) * 192, U * fc);
 #pragma unroll
@@ -736,6 +747,11 @@ __global__ __launch_bounds__(512, (Walk<DC, B16>::PAIR ? 4 : 2)) void k_delta_ch
             // ---- the state
             get(s_V, e[0]);
             get(s_V + 192, e[1]);
+            if (LATE && L::BUFFERS == 2) {
+#pragma unroll
+                for (int j = 0; j < OWN; j++) read_keys(i + 1, j);
+                __builtin_amdgcn_sched_barrier(0);
+            }
 #pragma unroll
             for (int j = 0; j < OWN; j++) {
                 const int cc = w + 4 * j;
