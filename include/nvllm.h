@@ -143,10 +143,14 @@ void nvllm_expert_ff(float* out, int* choice, float* score, const float* in, con
  * [qk_heads][dim], v: rows of [heads][vdim], the first of token t at element t * q_ld, t * k_ld, t * v_ld; out [num_tokens][heads][vdim];
  * elem_bytes 4: fp32, 2: bf16 (out is rounded once).  g (logarithm of the decay, at most 0; -infinity empties the state) and beta: fp32
  * [num_tokens][heads].  A sequence's tokens lie side by side at consecutive positions.  States and all sums in fp32.
- * dim at most 256.  out and state overlap nothing else.  Enqueued on the library stream; workspaces are the library's own.  Host
- * arrays may be reused on return.  Returns 0 or a refusal (below; nothing is enqueued then): NVLLM_BAD_ARGUMENT for null pointers,
- * sizes that are not positive, strides shorter than a row, pointers that are not multiples of their elements; NVLLM_BAD_SIZE;
- * NVLLM_BAD_INDEX for a sequence id outside the slots, a negative position, a sequence whose tokens are apart; NVLLM_CAPTURED. */
+ * dim at most 256, heads and vdim at most 65,535, heads * vdim and the strides at most 2^23.  out and state overlap nothing else.
+ * Portions go in chunks of 64 tokens from some length on (8 to 60 tokens, by the batch's size), whose products run over whole chunks: a
+ * value that is not finite reaches results of up to 63 tokens in front of its own, of the same sequence and head.  Enqueued on the
+ * library stream; workspaces are the library's own.  Host arrays may be reused on return.
+ * Returns 0 or a refusal (below; nothing is enqueued then): NVLLM_BAD_ARGUMENT for null pointers, sizes that are not positive,
+ * strides shorter than a row, pointers that are not multiples of their elements; NVLLM_BAD_SIZE for sizes beyond the limits, another
+ * elem_bytes, heads that are no multiple of qk_heads, more sequences than a call's staging takes; NVLLM_BAD_INDEX for a sequence id
+ * outside the slots, a negative position, a sequence whose tokens are apart; NVLLM_NO_MEMORY; NVLLM_CAPTURED. */
 int nvllm_gated_delta(void* out, const void* q, const void* k, const void* v, const float* g, const float* beta, float* state, const int* seq_ids, const int* pos_arr,
                       int n_slots, float scale, float norm_eps, int qk_heads, int heads, int dim, int vdim, int q_ld, int k_ld, int v_ld, int elem_bytes, int num_tokens);
 

@@ -3,7 +3,9 @@
 // k_delta_step: token by token.  With the state S of before, a = S^T k, b = S^T q and c = k . q, the token's correction and result are
 //   u = beta (v - e^g a),   o = scale (e^g b + c u),   S <- e^g S + k u^T,
 // so one pass over S and one sum over its rows serve both.  A wave holds 32 value columns of a head's state in registers (a lane: 4
-// columns x NR rows), reads it once, goes through the portion's tokens and writes it once.
+// columns x NR rows: 8 lanes read 128 bytes of a row), reads it once, goes through the portion's tokens and writes it once.  Bound by
+// memory: 64 sequences, 32 heads of 128 x 128: 270 MB in 59.7 us, 4.5 TB/s where a copy of 1 GiB reaches 5.1; the smallest calls by
+// the launch and their trips to memory (4 heads of 64 x 64: 5.9 us).
 //
 // Portions of several tokens go in chunks of 64.  With G_t the sum of g up to token t of the chunk, k and q normed, S the state in front:
 //   A_ts = beta_t e^(G_t - G_s) k_t . k_s  for s < t,   T' = (I + A)^-1 diag(beta),   P_ts = scale e^(G_t - G_s) q_t . k_s  for s <= t,
@@ -342,6 +344,9 @@ constexpr int prepare_keys() { return std::max(4 * DC * (B16 ? 1 : 3) * 1024, CH
 template <int DC, bool B16>
 constexpr int prepare_lds() { return prepare_keys<DC, B16>() + CH * LD * 4 + CH * (8 + 4 + 4); }
 
+// A workgroup = (portion, chunk, head), four waves of 16 tokens each.  A and P by the matrix cores, A in LDS for the inverse, whose sums are of
+// 32-bit products.  Bound by memory where chunks are many: 4,096 of 128 dims in bf16 move 230 MB in 51 us; few take 7 to 8 us, the
+// inverse's substitutions, one behind the other.
 template <int DC, bool B16, bool STEPS>
 __global__ __launch_bounds__(256) void k_delta_prepare(DeltaChunks c) {
     constexpr int PARTS = B16 ? 1 : 3;
@@ -520,7 +525,10 @@ __global__ __launch_bounds__(256) void k_delta_prepare(DeltaChunks c) {
 //   4, 5, the results of 32 tokens each, from the state and U as the chain leaves them in LDS.
 //   6, 7 bring keys, values, T' and factors of coming chunks from memory, one or two chunks ahead, and lay them out in LDS: the chain
 //     itself asks memory for nothing.
-// Three barriers a chunk (a fourth where LDS holds one chunk's keys only).
+// Three barriers a chunk (a fourth where LDS holds one chunk's keys only).  Bound by the chain: a chunk of 128 x 128 in bf16 takes 1.7 us,
+// 3,400 clocks, in which LDS is busy for 1,750 (400 of them conflicts) and a SIMD's matrix core for 960; the exchanges and their barriers
+// cost the rest.  Without the results' waves it would take 2,800, without the loaders' work 100 less.  Sixteen columns are
+// the fewest that the products take: more workgroups for the same heads, each as long.
 //
 // A portion's chunks may be cut into segments that are walked side by side: scouts (RESULTS false) find out what a segment makes of an empty
 // state (the first one: of the portion's) and, for columns of the unit matrix, what becomes of a state over it, k_delta_join forms the
@@ -1164,12 +1172,12 @@ constexpr size_t CHUNK_MEMORY = (size_t)192 << 20;   // of the chunks' records a
 // the hundred fill the chip; a chunk costs 14 us (19 us in 32 bits) whatever its tokens, and 5 us (8 us) more for every 256 workgroups
 // behind the first.  Measured, token by token and by chunks, heads of 128 x 128 in bf16: 32 heads, 8 tokens 15.4 and 14.1 us ... 20.2 and
 // 14.2 for 12; eight sequences (2,048 workgroups), 16 tokens: 30 and 46, 24: 42 and 46, 32: 53 and 47; 32 sequences, 32 tokens: 139 and 162,
-// 48: 204 and 170.
+// 48: 204 and 170; beyond that both grow with the batch.
 constexpr int CHUNK_LEAST = 8;
 static int chunk_min(const Delta& a, const std::vector<int4>& spans, bool b16) {
     double wgs = 0;
     for (const int4& s : spans) wgs += s.y >= CHUNK_LEAST ? (double)a.H * cdiv(a.vdim, 16) : 0.0;
-    return (int)((b16 ? 1.0 : 1.5) * CHUNK_LEAST * sqrt(std::max(1.0, wgs / 256)));
+    return (int)((b16 ? 1.0 : 1.5) * CHUNK_LEAST * std::min(5.0, sqrt(std::max(1.0, wgs / 256))));
 }
 
 // Segments of the portions' chunks, walked side by side, where heads and columns alone leave most of the chip empty.  They cost another walk
