@@ -29,18 +29,18 @@ constexpr int DELTA_CHUNK = 64;
 // What a chunk's tokens need of each other, per (chunk, head): the operands of T' and P (six 16 x 32 tiles on and below the diagonal
 // each, three parts), then per token the factors a, b and c, then what is left of the state.
 constexpr int DELTA_PART = 1024, DELTA_TILE = 3 * DELTA_PART, DELTA_OPS = 12 * DELTA_TILE, DELTA_RECORD = DELTA_OPS + 1024;
-struct DeltaChunks {
-    Delta a;                    // queries and keys: dims padded with zeros to a multiple of 8, rows 16-byte aligned
+struct DeltaChunks {           // (what every workgroup asks for first lies together)
     char* mem;                  // [chunk of the launch][H] records
     const int* first;           // [n_spans] the launch's first chunk of each span; null: the ones here
-    int first_here[DELTA_SPANS];
     int from, most;             // chunks [from, from + most) of every span
     int step_waves;             // of portions behind the first n_spans, which go token by token beside the first chunks
     int segs, per_seg;          // segments of a portion's chunks of the launch at most, chunks of one
+    int out_four;               // out can be stored four elements at a time
     float* starts;              // [span][segs][H][dims][columns] states that segments start from, both padded ...
     float* trans;               // [span][segs][H][dims][dims] ... and what becomes of a state over a segment
-    bool out_four;              // out can be stored four elements at a time
     double bytes, flops;        // kernel timing
+    Delta a;                    // queries and keys: dims padded with zeros to a multiple of 8, rows 16-byte aligned
+    int first_here[DELTA_SPANS];
 };
 
 }  // namespace nvllm

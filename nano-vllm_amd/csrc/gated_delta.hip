@@ -4,8 +4,8 @@
 //   u = beta (v - e^g a),   o = scale (e^g b + c u),   S <- e^g S + k u^T,
 // so one pass over S and one sum over its rows serve both.  A wave holds 32 value columns of a head's state in registers (a lane: 4
 // columns x NR rows: 8 lanes read 128 bytes of a row), reads it once, goes through the portion's tokens and writes it once.  Bound by
-// memory: 64 sequences, 32 heads of 128 x 128: 270 MB in 59.7 us, 4.5 TB/s where a copy of 1 GiB reaches 5.1; the smallest calls by
-// the launch and their trips to memory (4 heads of 64 x 64: 5.9 us).
+// memory: 64 sequences, 32 heads of 128 x 128: 270 MB in 52.5 us, 5.1 TB/s as a copy of 1 GiB; the smallest calls by the launch and
+// their trips to memory (4 heads of 64 x 64: 5.8 us).
 //
 // Portions of several tokens go in chunks of 64.  With G_t the sum of g up to token t of the chunk, k and q normed, S the state in front:
 //   A_ts = beta_t e^(G_t - G_s) k_t . k_s  for s < t,   T' = (I + A)^-1 diag(beta),   P_ts = scale e^(G_t - G_s) q_t . k_s  for s <= t,
@@ -27,23 +27,36 @@ namespace nvllm {
 
 typedef unsigned int u2_t __attribute__((ext_vector_type(2)));
 
-// Four neighbouring elements as they lie in memory; in 32 bits each where the addresses are no multiples of four elements.
+// Memory by descriptors: what lies behind `bytes` (and every offset of NOWHERE) reads as zeros and is not written, so that a chunk's
+// loads have no branch around them and all of them are in flight together.
+constexpr unsigned NOWHERE = 0x80000000u;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t memory(const void* base, long bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)bytes, 0x00020000);
+}
+__device__ __forceinline__ u4_t load16(__amdgpu_buffer_rsrc_t m, unsigned at, int base = 0) { return __builtin_bit_cast(u4_t, __builtin_amdgcn_raw_buffer_load_b128(m, (int)at, base, 0)); }
+__device__ __forceinline__ float load4(__amdgpu_buffer_rsrc_t m, unsigned at) { return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(m, (int)at, 0, 0)); }
+__device__ __forceinline__ unsigned two_b16(float lo, float hi) {
+    typedef __bf16 b2_t __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(unsigned, b2_t{(__bf16)lo, (__bf16)hi});
+}
+// Four neighbouring elements as they lie in memory, of which the first `left` are there; one by one where the addresses are no multiples of
+// four elements.
 template <bool B16, bool VEC>
 struct Four {
     u4_t w;
-    __device__ __forceinline__ void load(const void* base, size_t at, int left) {
+    template <int AUX = 0>
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t m, unsigned at, int left) {
         if (VEC) {
-            if (left <= 0) w = u4_t{0, 0, 0, 0};
-            else if (B16) {
-                const u2_t p = *reinterpret_cast<const u2_t*>((const unsigned short*)base + at);
+            const int from = (int)(left > 0 ? at : NOWHERE);
+            if (B16) {
+                const u2_t p = __builtin_amdgcn_raw_buffer_load_b64(m, from, 0, AUX);
                 w = u4_t{p[0], p[1], 0, 0};
-            } else w = *reinterpret_cast<const u4_t*>((const float*)base + at);
+            } else w = __builtin_bit_cast(u4_t, __builtin_amdgcn_raw_buffer_load_b128(m, from, 0, AUX));
         } else {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                if (i >= left) w[i] = 0;
-                else if (B16) w[i] = (unsigned)((const unsigned short*)base)[at + i] << 16;
-                else w[i] = ((const unsigned*)base)[at + i];
+                if (B16) w[i] = (unsigned)(unsigned short)__builtin_amdgcn_raw_buffer_load_b16(m, (int)(i < left ? at + 2 * i : NOWHERE), 0, AUX) << 16;
+                else w[i] = __builtin_amdgcn_raw_buffer_load_b32(m, (int)(i < left ? at + 4 * i : NOWHERE), 0, AUX);
             }
         }
     }
@@ -54,21 +67,19 @@ struct Four {
         return __builtin_bit_cast(f4_t, w);
     }
 };
-template <bool B16, bool VEC>
-__device__ __forceinline__ void store_four(void* base, size_t at, const f4_t& v, int left) {
+template <bool B16, bool VEC, int AUX = 0>
+__device__ __forceinline__ void store_four(__amdgpu_buffer_rsrc_t m, unsigned at, const f4_t& v, int left) {
     if (VEC) {
-        if (left <= 0) return;
-        if (B16) {
-            typedef __bf16 b4_t __attribute__((ext_vector_type(4)));
-            *reinterpret_cast<b4_t*>((__bf16*)base + at) = b4_t{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
-        } else *reinterpret_cast<f4_t*>((float*)base + at) = v;
+        const int to = (int)(left > 0 ? at : NOWHERE);
+        if (B16) __builtin_amdgcn_raw_buffer_store_b64(u2_t{two_b16(v[0], v[1]), two_b16(v[2], v[3])}, m, to, 0, AUX);
+        else __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4_t, v), m, to, 0, AUX);
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (i < left) {
-                if (B16) ((__bf16*)base)[at + i] = (__bf16)v[i];
-                else ((float*)base)[at + i] = v[i];
-            }
+        for (int i = 0; i < 4; i++) {
+            const float z = v[i];
+            if (B16) __builtin_amdgcn_raw_buffer_store_b16((unsigned short)two_b16(z, z), m, (int)(i < left ? at + 2 * i : NOWHERE), 0, AUX);
+            else __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, z), m, (int)(i < left ? at + 4 * i : NOWHERE), 0, AUX);
+        }
     }
 }
 // e^g, the product with log2(e) in 64 bits: its rounding would count for large |g|
@@ -86,37 +97,56 @@ __device__ __forceinline__ float sum_over_rows(float x) {
 
 constexpr int STEP_COLS = 32;   // of a wave
 
+// A kernel's arguments come from memory, and each is asked for where it is first used: one trip behind the other before the first load of
+// data.  Named together in front they take one trip.
+#define ASKED_FOR_AT_ONCE(A)                                                                                                                            \
+    asm volatile("" ::"s"((A).q), "s"((A).k), "s"((A).v), "s"((A).g), "s"((A).beta), "s"((A).state), "s"((A).q_ld), "s"((A).k_ld), "s"((A).v_ld), "s"((A).H), "s"((A).Q), \
+                 "s"((A).dim), "s"((A).vdim), "s"((A).spans), "s"((A).eps), "s"((A).scale))
+__device__ __forceinline__ int4 scalars(const int4& v) {
+    return int4{__builtin_amdgcn_readfirstlane(v.x), __builtin_amdgcn_readfirstlane(v.y), __builtin_amdgcn_readfirstlane(v.z), __builtin_amdgcn_readfirstlane(v.w)};
+}
+// a portion of the launch, in scalar registers
+__device__ __forceinline__ int4 span_of(const Delta& a, int s) {
+    int4 v = a.here[min(s, DELTA_SPANS - 1)];
+    ASKED_FOR_AT_ONCE(a);
+    asm volatile("" ::"s"(v.x), "s"(v.y), "s"(v.z), "s"(v.w));
+    if (a.spans) v = a.spans[s];
+    return scalars(v);
+}
+
 template <bool B16, int NR, bool VEC>
-__device__ __forceinline__ void delta_step(const Delta& a, int idx, int lane) {   // idx = (portion, head, slice) of the wave
+__device__ __forceinline__ void delta_step(const Delta& a, const int4& span, int h, int slice, int lane) {   // portion, head and slice of the wave
     constexpr int R4 = NR / 4;
     typedef Four<B16, VEC> F;
-    const int slices = (a.vdim + STEP_COLS - 1) / STEP_COLS;
-    const int slice = idx % slices;
-    idx /= slices;
-    const int h = idx % a.H;
-    const int4 span = (a.spans ? a.spans : a.here)[idx / a.H];
     const int col = slice * STEP_COLS + (lane & 7) * 4, row0 = (lane >> 3) * NR, hq = h / (a.H / a.Q);
-    const int cols = a.vdim - col, rows = a.dim - row0;   // that this lane has at most
+    constexpr int ELEM = B16 ? 2 : 4;
+    const int cols = a.vdim - col;   // that this lane has at most
+    // Rows behind the last one lie behind the descriptors' ends.  States are read once and written once, past the caches, which other layers'
+    // states pass through before they are back: twelve layers in turn, 64 sequences, 32 heads of 128 x 128: 59.1 us through the caches, 53.5
+    // past them; of 64 x 64: 17.5, 14.1.  (Three layers that fit the caches: 32 sequences of 128 x 128 22.6, 27.8.)
+    constexpr int PAST = 2;
     float* st = a.state + ((size_t)span.w * a.H + h) * a.dim * a.vdim;
+    const long st_bytes = (long)a.dim * a.vdim * 4;
+    const unsigned st_at = ((unsigned)row0 * a.vdim + col) * 4, st_row = 4u * a.vdim;
     f4_t S[NR];
+    {
+        const auto m = memory(st, span.z > 0 ? st_bytes : 0);
+        Four<false, VEC> in[NR];
 #pragma unroll
-    for (int r = 0; r < NR; r++) {
-        S[r] = f4_t{0.f, 0.f, 0.f, 0.f};
-        if (span.z > 0 && r < rows) {
-            Four<false, VEC> w;
-            w.load(st, (size_t)(row0 + r) * a.vdim + col, cols);
-            S[r] = w.get();
-        }
+        for (int r = 0; r < NR; r++) in[r].template load<PAST>(m, st_at + r * st_row, cols);
+#pragma unroll
+        for (int r = 0; r < NR; r++) S[r] = in[r].get();
     }
     F kn[R4], qn[R4], vn;
     float gn, bn;
     auto fetch = [&](int t) {
+        const auto mk = memory((const char*)a.k + ((size_t)t * a.k_ld + hq * a.dim) * ELEM, a.dim * ELEM), mq = memory((const char*)a.q + ((size_t)t * a.q_ld + hq * a.dim) * ELEM, a.dim * ELEM);
 #pragma unroll
         for (int r = 0; r < R4; r++) {
-            kn[r].load(a.k, (size_t)t * a.k_ld + hq * a.dim + row0 + 4 * r, rows - 4 * r);
-            qn[r].load(a.q, (size_t)t * a.q_ld + hq * a.dim + row0 + 4 * r, rows - 4 * r);
+            kn[r].load(mk, (row0 + 4 * r) * ELEM, a.dim - row0 - 4 * r);
+            qn[r].load(mq, (row0 + 4 * r) * ELEM, a.dim - row0 - 4 * r);
         }
-        vn.load(a.v, (size_t)t * a.v_ld + h * a.vdim + col, cols);
+        vn.load(memory((const char*)a.v + ((size_t)t * a.v_ld + h * a.vdim) * ELEM, a.vdim * ELEM), col * ELEM, cols);
         gn = a.g[(size_t)t * a.H + h];
         bn = a.beta[(size_t)t * a.H + h];
     };
@@ -168,19 +198,22 @@ __device__ __forceinline__ void delta_step(const Delta& a, int idx, int lane) { 
         for (int r = 0; r < NR; r++)
 #pragma unroll
             for (int e = 0; e < 4; e++) S[r][e] = fmaf(k[r / 4][r % 4], u[e], decay * S[r][e]);
-        if (lane < 8) store_four<B16, VEC>(a.out, ((size_t)t * a.H + h) * a.vdim + col, o, cols);
+        store_four<B16, VEC>(memory((const char*)a.out + ((size_t)t * a.H + h) * a.vdim * ELEM, a.vdim * ELEM), col * ELEM, o, lane < 8 ? cols : 0);
     }
 #pragma unroll
-    for (int r = 0; r < NR; r++)
-        if (r < rows) store_four<false, VEC>(st, (size_t)(row0 + r) * a.vdim + col, S[r], cols);
+    for (int r = 0; r < NR; r++) store_four<false, VEC, PAST>(memory(st, st_bytes), st_at + r * st_row, S[r], cols);
 }
 
 template <bool B16, int NR, bool VEC>
-__global__ __launch_bounds__(64) void k_delta_step(Delta a) { delta_step<B16, NR, VEC>(a, blockIdx.x, threadIdx.x); }
+__global__ __launch_bounds__(64) void k_delta_step(Delta a) {
+    const int4 span = span_of(a, blockIdx.y);
+    const int slices = (a.vdim + STEP_COLS - 1) / STEP_COLS, h = blockIdx.x / slices;
+    delta_step<B16, NR, VEC>(a, span, h, blockIdx.x - h * slices, threadIdx.x);
+}
 
 template <bool B16, bool VEC>
 static void launch_step(const Delta& a) {
-    const dim3 grid((unsigned)(cdiv(a.vdim, STEP_COLS) * a.H * a.n_spans));
+    const dim3 grid((unsigned)(cdiv(a.vdim, STEP_COLS) * a.H), a.n_spans);
     const int nr = cdiv(a.dim, 8);
     if (nr <= 4) NVLLM_LAUNCH((k_delta_step<B16, 4, VEC>), grid, dim3(64), 0, a);
     else if (nr <= 8) NVLLM_LAUNCH((k_delta_step<B16, 8, VEC>), grid, dim3(64), 0, a);
@@ -199,10 +232,6 @@ constexpr float MIN_G = -1e4f;   // e^MIN_G is zero, and differences of sums of 
 // x = a + b + c, each rounded to the nearest bf16 of what is left: exact but for the 26th bit, and what a product of two leaves out has no
 // sign of its own.  (Truncations, of the factors' own signs, left a bias: sums of 64 corrections to one key were off by 520 halves
 // of a step.)
-__device__ __forceinline__ unsigned two_b16(float lo, float hi) {
-    typedef __bf16 b2_t __attribute__((ext_vector_type(2)));
-    return __builtin_bit_cast(unsigned, b2_t{(__bf16)lo, (__bf16)hi});
-}
 __device__ __forceinline__ u2_t next_part(f4_t& v) {   // the part of four values, and what it leaves of them
     u2_t p = {two_b16(v[0], v[1]), two_b16(v[2], v[3])};
     asm("" : "+v"(p));   // (the upper halves come from these registers, not from roundings of their own)
@@ -261,15 +290,6 @@ __device__ __forceinline__ double sum_up_to(double x, int lane) {
     return x + (lane < 16 ? 0.0 : lane < 32 ? r0 : lane < 48 ? r1 : r2);
 }
 
-// Memory by descriptors: what lies behind `bytes` (and every offset of NOWHERE) reads as zeros and is not written, so that a chunk's
-// loads have no branch around them and all of them are in flight together.
-constexpr unsigned NOWHERE = 0x80000000u;
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t memory(const void* base, long bytes) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)bytes, 0x00020000);
-}
-__device__ __forceinline__ u4_t load16(__amdgpu_buffer_rsrc_t m, unsigned at, int base = 0) { return __builtin_bit_cast(u4_t, __builtin_amdgcn_raw_buffer_load_b128(m, (int)at, base, 0)); }
-__device__ __forceinline__ float load4(__amdgpu_buffer_rsrc_t m, unsigned at) { return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(m, (int)at, 0, 0)); }
-
 // A token's row of queries or keys as operands: lane (x, g) has dims 32 cc + 8 g .. + 7 of the tile's row x.
 template <int DC, bool B16>
 struct Rows {
@@ -315,12 +335,20 @@ __device__ __forceinline__ f4_t mfma_rows(const b8_t (&a)[B16 ? 1 : 3], const b8
     else return mfma6(a, b, c);
 }
 
-// a portion of the launch, and its first record, in scalar registers
-__device__ __forceinline__ int4 span_of(const Delta& a, int s) {
-    const int4 v = a.spans ? a.spans[s] : a.here[s];
-    return int4{__builtin_amdgcn_readfirstlane(v.x), __builtin_amdgcn_readfirstlane(v.y), __builtin_amdgcn_readfirstlane(v.z), __builtin_amdgcn_readfirstlane(v.w)};
+// ... and its first record
+struct Portion {
+    int4 span;
+    int first;
+};
+__device__ __forceinline__ Portion portion_of(const DeltaChunks& c, int s) {
+    const int at = min(s, DELTA_SPANS - 1);
+    Portion p = {c.a.here[at], c.first_here[at]};
+    ASKED_FOR_AT_ONCE(c.a);
+    asm volatile("" ::"s"(p.span.x), "s"(p.span.y), "s"(p.span.z), "s"(p.span.w), "s"(p.first), "s"(c.mem), "s"(c.first), "s"(c.from), "s"(c.most), "s"(c.segs), "s"(c.per_seg), "s"(c.out_four),
+                 "s"(c.a.out), "s"(c.a.v_cols), "s"(c.a.dim_kept));
+    if (c.a.spans) p = {c.a.spans[s], c.first[s]};
+    return {scalars(p.span), __builtin_amdgcn_readfirstlane(p.first)};
 }
-__device__ __forceinline__ int first_of(const DeltaChunks& c, int s) { return __builtin_amdgcn_readfirstlane(c.first ? c.first[s] : c.first_here[s]); }
 struct ChunkAt {
     int4 span;
     int first, n;   // token of the batch, tokens
@@ -328,10 +356,11 @@ struct ChunkAt {
 };
 __device__ __forceinline__ ChunkAt chunk_at(const DeltaChunks& c, int s, int h, int i) {
     ChunkAt at;
-    at.span = span_of(c.a, s);
+    const Portion p = portion_of(c, s);
+    at.span = p.span;
     at.first = at.span.x + (c.from + i) * CH;
     at.n = min(CH, at.span.y - (c.from + i) * CH);
-    at.record = c.mem + ((size_t)(first_of(c, s) + i) * c.a.H + h) * DELTA_RECORD;
+    at.record = c.mem + ((size_t)(p.first + i) * c.a.H + h) * DELTA_RECORD;
     return at;
 }
 // T' and P: tile (token tile w, 32 tokens p) of the six that are not empty
@@ -360,11 +389,15 @@ __global__ __launch_bounds__(256) void k_delta_prepare(DeltaChunks c) {
     const Delta& a = c.a;
     if (STEPS && (int)blockIdx.z >= a.n_spans) {   // portions that go token by token, behind the others
         const int wave = (((blockIdx.z - a.n_spans) * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        if (wave < c.step_waves) delta_step<B16, 4 * DC, true>(a, a.n_spans * a.H * ((a.vdim + STEP_COLS - 1) / STEP_COLS) + wave, threadIdx.x & 63);
+        if (wave < c.step_waves) {
+            const int slices = (a.vdim + STEP_COLS - 1) / STEP_COLS, i = wave / slices, s = i / a.H;
+            delta_step<B16, 4 * DC, true>(a, span_of(a, a.n_spans + s), i - s * a.H, wave - i * slices, threadIdx.x & 63);
+        }
         return;
     }
-    const int h = blockIdx.x, hq = h / (a.H / a.Q);
+    const int h = blockIdx.x;
     const ChunkAt at = chunk_at(c, blockIdx.z, h, blockIdx.y);
+    const int hq = h / (a.H / a.Q);
     if (at.n <= 0) return;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), x = lane & 15, g = lane >> 4;
     const int t = 16 * w + x;
@@ -559,16 +592,22 @@ __global__ __launch_bounds__(512, (Walk<DC, B16>::PAIR ? 4 : 2)) void k_delta_ch
     u4_t* s_k = reinterpret_cast<u4_t*>(s_f + 256);        // [buffer][DC][part][token][4] keys, 32 dims together
     u4_t* s_t = s_k + L::BUFFERS * DC * PARTS * 256;       // T', and a tile of zeros
     const Delta& a = c.a;
-    const int h = blockIdx.x, hq = h / (a.H / a.Q), of = blockIdx.z / c.segs, seg = blockIdx.z - of * c.segs;
+    int of = blockIdx.z;
+    Portion portion = portion_of(c, of);
+    if (c.segs > 1) {
+        of = blockIdx.z / c.segs;
+        portion = portion_of(c, of);
+    }
+    const int h = blockIdx.x, hq = h / (a.H / a.Q), seg = blockIdx.z - of * c.segs;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), x = lane & 15, g = lane >> 4;
-    const int4 span = span_of(a, of);
+    const int4 span = portion.span;
     const int all = min(c.most, (span.y + CH - 1) / CH - c.from), c0 = seg * c.per_seg, chunks = min(c.per_seg, all - c0);
     const int slices = (a.vdim + 15) / 16;
     const bool unit = !RESULTS && (int)blockIdx.y >= slices;   // columns of the unit matrix
     if (chunks <= 0 || (!RESULTS && (c0 + chunks >= all || (unit && seg == 0)))) return;
     const int slice = unit ? blockIdx.y - slices : blockIdx.y;
     const int first = span.x + (c.from + c0) * CH, tokens = min(span.y - (c.from + c0) * CH, chunks * CH);
-    const char* record = c.mem + ((size_t)(first_of(c, of) + c0) * a.H + h) * DELTA_RECORD;
+    const char* record = c.mem + ((size_t)(portion.first + c0) * a.H + h) * DELTA_RECORD;
     auto rows_of = [&](const void* base, long ld, int at, int i, int width) {   // of chunk i's tokens; behind the last chunk: the last one's
         const int ci = min(i, chunks - 1), n = min(CH, tokens - ci * CH);
         return memory((const char*)base + ((size_t)(first + ci * CH) * ld + at) * ELEM, ((n - 1) * ld + width) * ELEM);
@@ -894,7 +933,10 @@ __global__ __launch_bounds__(512, (Walk<DC, B16>::PAIR ? 4 : 2)) void k_delta_ch
             meet(DC / 2, DC);
             f4_t now[2];
 #pragma unroll
-            for (int t = 0; t < 2; t++) now[t] = (O[t][0] + O[t][1]) * mine.fb[t];
+            for (int t = 0; t < 2; t++) {
+                now[t] = (O[t][0] + O[t][1]) * mine.fb[t];
+                asm volatile("" : "+v"(now[t]));   // (here, not behind the branch below)
+            }
             fetch_queries(mine, i + SETS);
             __syncthreads();
             if (L::BUFFERS == 1) __syncthreads();   // U is there
@@ -1309,6 +1351,8 @@ static int gated_delta(Delta& a, const int* seq_ids, const int* pos, int T, int 
         const long waves = (long)cdiv(a.vdim, STEP_COLS) * a.H * ((long)spans.size() - n_chunked);
         if (fits && v_fits && vec && (!b16 || n_records * a.H <= 4 * (size_t)rt().num_cus) && n_chunked + waves / (4L * a.H * most) < 65535) {
             c.step_waves = (int)waves;
+            c.bytes += (states[0] + (double)(T - tokens) * token_bytes) / rounds;
+            c.flops += (double)(T - tokens) * token_flops / rounds;
             a.n_spans = 0;
         }
         for (c.from = 0; c.from < longest; c.from += most) {
@@ -1322,10 +1366,13 @@ static int gated_delta(Delta& a, const int* seq_ids, const int* pos, int T, int 
     a.spans = d_spans ? d_spans + n_chunked : nullptr;
     if (!d_spans) std::copy(spans.begin() + n_chunked, spans.end(), a.here);
     ProfScope ps(PC_DELTA_TOK, states[0] + (double)(T - tokens) * token_bytes, (double)(T - tokens) * token_flops);
-    if (b16 && vec) launch_step<true, true>(a);
-    else if (b16) launch_step<true, false>(a);
-    else if (vec) launch_step<false, true>(a);
-    else launch_step<false, false>(a);
+    for (int left = a.n_spans; left > 0; left -= a.n_spans, a.spans += a.n_spans) {   // (what a grid takes)
+        a.n_spans = std::min(left, 65535);
+        if (b16 && vec) launch_step<true, true>(a);
+        else if (b16) launch_step<true, false>(a);
+        else if (vec) launch_step<false, true>(a);
+        else launch_step<false, false>(a);
+    }
     return 0;
 }
 
