@@ -144,7 +144,7 @@ void nvllm_expert_ff(float* out, int* choice, float* score, const float* in, con
  * elem_bytes 4: fp32, 2: bf16 (out is rounded once).  g (logarithm of the decay, at most 0; -infinity empties the state) and beta: fp32
  * [num_tokens][heads].  A sequence's tokens lie side by side at consecutive positions.  States and all sums in fp32.
  * dim at most 256, heads and vdim at most 65,535, heads * vdim and the strides at most 2^23.  out and state overlap nothing else.
- * Portions go in chunks of 64 tokens from some length on (8 to 60 tokens, by the batch's size), whose products run over whole chunks: a
+ * Portions go in chunks of 64 tokens from some length on (10 to 75 tokens, by the batch's size and type), whose products run over whole chunks: a
  * value that is not finite reaches results of up to 63 tokens in front of its own, of the same sequence and head.  Enqueued on the
  * library stream; workspaces are the library's own.  Host arrays may be reused on return.
  * Returns 0 or a refusal (below; nothing is enqueued then): NVLLM_BAD_ARGUMENT for null pointers, sizes that are not positive,

@@ -1210,12 +1210,12 @@ static int delta_spans(std::vector<int4>& spans, const int* seq_ids, const int* 
 
 constexpr size_t CHUNK_MEMORY = (size_t)192 << 20;   // of the chunks' records at a time
 
-// Tokens from which a portion goes by chunks.  A token of a portion costs 1.2 us on the way token by token (128 dims), 4 us where states by
-// the hundred fill the chip; a chunk costs 14 us (19 us in 32 bits) whatever its tokens, and 5 us (8 us) more for every 256 workgroups
-// behind the first.  Measured, token by token and by chunks, heads of 128 x 128 in bf16: 32 heads, 8 tokens 15.4 and 14.1 us ... 20.2 and
-// 14.2 for 12; eight sequences (2,048 workgroups), 16 tokens: 30 and 46, 24: 42 and 46, 32: 53 and 47; 32 sequences, 32 tokens: 139 and 162,
-// 48: 204 and 170; beyond that both grow with the batch.
-constexpr int CHUNK_LEAST = 8;
+// Tokens from which a portion goes by chunks.  A token of a portion costs 1 us on the way token by token (128 dims), 3.3 us where states by
+// the hundred fill the chip; a chunk costs 13 us (18 us in 32 bits) whatever its tokens, and 5 us (8 us) more for every 256 workgroups
+// behind the first.  Measured, token by token and by chunks, heads of 128 x 128 in bf16: 32 heads, 8 tokens 11.3 and 12.9 us, 12 tokens 15.5
+// and 13.1; eight sequences (2,048 workgroups), 32 tokens: 40 and 46, 48: 58 and 48; 32 sequences, 32 tokens: 105 and 162, 48: 156
+// and 167; beyond that both grow with the batch.
+constexpr int CHUNK_LEAST = 10;
 static int chunk_min(const Delta& a, const std::vector<int4>& spans, bool b16) {
     double wgs = 0;
     for (const int4& s : spans) wgs += s.y >= CHUNK_LEAST ? (double)a.H * cdiv(a.vdim, 16) : 0.0;
@@ -1344,12 +1344,11 @@ static int gated_delta(Delta& a, const int* seq_ids, const int* pos, int T, int 
         const int rounds = cdiv(longest, most);
         c.bytes = (states[1] + (double)tokens * token_bytes) / rounds;
         c.flops = (double)tokens * token_flops / rounds;
-        // The others' steps go with the first chunks' launch where rows are aligned for both, unless there are chunks for several turns on
-        // every CU, which then run fewer at a time (in 16 bits; in 32 they take as many registers as the steps).  Apart and together:
-        // three portions of 512 tokens and eleven of one, 32 heads of 64 x 64: 40.0 us, 36.8; one of 512 and 64, 128 x 128: 94, 84 (in
-        // 32 bits 111, 98); four of 1,024 and 64: 226, 230 (362, 347).
+        // The others' steps go with the first chunks' launch where rows are aligned for both.  Apart and together: three portions of 512 tokens
+        // and eleven of one, 32 heads of 64 x 64: 36.5 us, 32.0; one of 512 and 64, 128 x 128: 83, 72 (in 32 bits 101, 89); four of 1,024
+        // and 64: 207, 199 (350, 340).
         const long waves = (long)cdiv(a.vdim, STEP_COLS) * a.H * ((long)spans.size() - n_chunked);
-        if (fits && v_fits && vec && (!b16 || n_records * a.H <= 4 * (size_t)rt().num_cus) && n_chunked + waves / (4L * a.H * most) < 65535) {
+        if (fits && v_fits && vec && n_chunked + waves / (4L * a.H * most) < 65535) {
             c.step_waves = (int)waves;
             c.bytes += (states[0] + (double)(T - tokens) * token_bytes) / rounds;
             c.flops += (double)(T - tokens) * token_flops / rounds;

@@ -122,7 +122,7 @@ def test_a_long_portion(hip, elem):
 
 
 @BOTH
-@pytest.mark.parametrize("n", [6, 7, 8, 9, 11, 12, 13, 22, 23, 33, 34])
+@pytest.mark.parametrize("n", [6, 7, 8, 9, 10, 11, 12, 13, 14, 15, 22, 23, 28, 29, 33, 34, 42, 43])
 def test_short_portions(hip, elem, n):
     """About the lengths at which chunks take over, which rise with the batch."""
     check(hip, elem, [(1, 0, n), (0, 60, n + 1)], 2, 2, 64, 48)
