@@ -374,7 +374,7 @@ template <int DC, bool B16>
 constexpr int prepare_lds() { return prepare_keys<DC, B16>() + CH * LD * 4 + CH * (8 + 4 + 4); }
 
 // A workgroup = (portion, chunk, head), four waves of 16 tokens each.  A and P by the matrix cores, A in LDS for the inverse, whose sums are of
-// 32-bit products.  Bound by memory where chunks are many: 4,096 of 128 dims in bf16 move 230 MB in 51 us; few take 7 to 8 us, the
+// 32-bit products.  Bound by memory where chunks are many: 4,096 of 128 dims in bf16 move 230 MB in 50 us; few take 7 to 8 us, the
 // inverse's substitutions, one behind the other.
 template <int DC, bool B16, bool STEPS>
 __global__ __launch_bounds__(256) void k_delta_prepare(DeltaChunks c) {
@@ -558,9 +558,9 @@ __global__ __launch_bounds__(256) void k_delta_prepare(DeltaChunks c) {
 //   4, 5, the results of 32 tokens each, from the state and U as the chain leaves them in LDS.
 //   6, 7 bring keys, values, T' and factors of coming chunks from memory, one or two chunks ahead, and lay them out in LDS: the chain
 //     itself asks memory for nothing.
-// Three barriers a chunk (a fourth where LDS holds one chunk's keys only).  Bound by the chain: a chunk of 128 x 128 in bf16 takes 1.7 us,
-// 3,400 clocks, in which LDS is busy for 1,750 (400 of them conflicts) and a SIMD's matrix core for 960; the exchanges and their barriers
-// cost the rest.  Without the results' waves it would take 2,800, without the loaders' work 100 less.  Sixteen columns are
+// Three barriers a chunk (a fourth where LDS holds one chunk's keys only).  Bound by the chain: a chunk of 128 x 128 in bf16 takes 1.6 us,
+// 3,300 clocks, in which LDS is busy for 1,750 (400 of them conflicts) and a SIMD's matrix core for 960; the exchanges and their barriers
+// cost the rest.  The results' waves add a fifth to what the chain would take alone, the loaders' work 4 %.  Sixteen columns are
 // the fewest that the products take: more workgroups for the same heads, each as long.
 //
 // A portion's chunks may be cut into segments that are walked side by side: scouts (RESULTS false) find out what a segment makes of an empty
@@ -1225,8 +1225,8 @@ static int chunk_min(const Delta& a, const std::vector<int4>& spans, bool b16) {
 // Segments of the portions' chunks, walked side by side, where heads and columns alone leave most of the chip empty.  They cost another walk
 // for what a segment does to a state (its scouts), of which as many run at a time as there are CUs, and a join in which one start waits for
 // the other; n segments of m chunks take about m / n + DC n / 2.5 of a chunk's time, least at sqrt(2.5 m / DC).  Measured, in one segment and
-// in this many: 8,192 tokens, one head of 128 x 128: 212 us, 87 in 8; four: 212, 109 in 5; eight: 218, 154 in 3 (166 in 4, which no longer fit
-// side by side); one of 64 x 64: 201, 69 in 12; 4,096 tokens, two of 256 x 256: 157, 119 in 4; 1,024 tokens, one of 128 x 128: 38, 41 in 3.
+// in this many: 8,192 tokens, one head of 128 x 128: 194 us, 83 in 8; four: 195, 105 in 5; eight: 201, 146 in 3 (161 in 4, which no longer
+// fit side by side); one of 64 x 64: 174, 58 in 12; 4,096 tokens, two of 256 x 256: 157, 117 in 4; 1,024 tokens, one of 128 x 128: 35, 39 in 3.
 static void delta_segments(DeltaChunks& c, int DC, int most) {
     const Delta& a = c.a;
     const long walks = (long)a.H * cdiv(a.vdim, 16) * a.n_spans, unit = (long)a.H * 2 * DC * a.n_spans, cus = rt().num_cus;
