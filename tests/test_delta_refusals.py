@@ -44,5 +44,16 @@ def test_batches(lib, over):
     assert call(lib, **over) == BAD_INDEX
 
 
+@pytest.mark.parametrize("over", [dict(q_ld=2 ** 23 + 1), dict(v_ld=2 ** 23 + 8), dict(heads=2 ** 12, qk_heads=2 ** 12, dim=1, q_ld=2 ** 12, k_ld=2 ** 12, vdim=2 ** 12, v_ld=2 ** 23),
+                                  dict(vdim=65536, heads=2, v_ld=2 ** 17)], ids=str)
+def test_limits(lib, over):
+    assert call(lib, **over) == BAD_SIZE
+
+
+def test_more_sequences_than_a_call_takes(lib):
+    n = 220000
+    assert call(lib, ids=range(n), pos=[3] * n, n_slots=n, tokens=n) == BAD_SIZE
+
+
 def test_no_tokens_is_no_call(lib):
     assert call(lib, tokens=0, out=None, ids=None) == 0

@@ -275,6 +275,11 @@ def test_portions_beside_single_tokens(hip, elem, heads):
 
 
 @BOTH
+def test_more_sequences_than_a_grid_takes(hip, elem):
+    check(hip, elem, [(70000 - i, i % 3, 1) for i in range(70000)], 1, 1, 4, 4)
+
+
+@BOTH
 def test_samples_and_beams_of_one_prompt(hip, elem):
     """As a program uses the two together: a prompt, its state to the samples' slots, then steps before each of which every sample goes on from
     the state of a chosen one."""
