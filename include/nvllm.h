@@ -158,7 +158,9 @@ int nvllm_gated_delta(void* out, const void* q, const void* k, const void* v, co
 /* No counterpart in the reference, whose sequences never share or move anything.  A sequence that branches (several samples of
  * one prompt, beams) takes its past along: the table of its blocks by nvllm_fork_tables, and its states, if it has some, by
  * nvllm_copy_states or nvllm_copy_model_states.  Like every operator these enqueue on the library stream, so they come behind the
- * passes that were enqueued before and in front of later ones; the host's records change at once.
+ * passes that were enqueued before and in front of later ones; the host's records change at once.  Pools and tables are the
+ * caller's to guard: threads that each keep a pool of their own may call what enqueues nothing (forks of whole blocks, releases,
+ * alloc_block and free_block) at the same time.
  *
  * What these entry points and nvllm_gated_delta answer when they refuse.  A call that refuses changes nothing. */
 enum {

@@ -4,6 +4,7 @@
 #include <algorithm>
 #include <array>
 #include <cstring>
+#include <mutex>
 #include <new>
 #include <unordered_map>
 #include <vector>
@@ -16,6 +17,13 @@
 #include "step_arrays.h"
 
 namespace nvllm {
+
+// What is known of pools may be asked for by threads that each keep a pool of their own.
+static std::mutex& pools_lock() {
+    static std::mutex m;
+    return m;
+}
+#define WITH_POOLS std::lock_guard<std::mutex> with_pools(pools_lock())
 
 // Pools created by init_kv_cache_manager, keyed by pool_k: element size and the
 // geometry the reference passes again with every call.
@@ -34,6 +42,7 @@ static std::unordered_map<const void*, BlockPool>& block_pools() {
     return m;
 }
 size_t block_pool_bytes(const KVCacheManager* mgr) {
+    WITH_POOLS;
     auto it = block_pools().find(mgr->pool_k);
     return it == block_pools().end() ? 0 : it->second.bytes;
 }
@@ -44,6 +53,7 @@ static std::unordered_map<const void*, PoolInfo>& pools() {
 }
 
 std::vector<SlotArrays> pool_arrays(const KVCacheManager* mgr) {
+    WITH_POOLS;
     const auto own = block_pools().find(mgr->pool_k);
     if (own != block_pools().end()) return own->second.arrays;
     const auto it = pools().find(mgr->pool_k);
@@ -57,8 +67,11 @@ KvPoolView pool_view(const KVCacheManager* mgr, int n_kv_heads, int head_dim) {
     KvPoolView v;
     v.k = mgr->pool_k;
     v.v = mgr->pool_v;
-    auto it = pools().find(mgr->pool_k);
-    v.elem_bytes = it == pools().end() ? 4 : it->second.elem_bytes;
+    {
+        WITH_POOLS;
+        auto it = pools().find(mgr->pool_k);
+        v.elem_bytes = it == pools().end() ? 4 : it->second.elem_bytes;
+    }
     v.block_size = mgr->block_size;
     v.num_blocks = mgr->num_blocks;
     v.layer_stride = (long)mgr->num_blocks * mgr->block_size * n_kv_heads * head_dim;
@@ -395,6 +408,7 @@ void init_kv_cache_manager(KVCacheManager* mgr, int block_size, int num_blocks, 
     HIP_CHECK(hipMemsetAsync(pv, 0, elems * eb, rt().stream));
     mgr->pool_k = (float*)pk;
     mgr->pool_v = (float*)pv;
+    WITH_POOLS;
     pools()[pk] = PoolInfo{eb, n_layers, n_kv_heads, head_dim, true};
 }
 
@@ -403,10 +417,11 @@ int nvllm_attach_kv_pool(KVCacheManager* mgr, int block_size, int num_blocks, in
     if (elem_bytes != 2 && elem_bytes != 4) return NVLLM_BAD_SIZE;
     if (elem_bytes == 2 && (block_size != KV16_PAGE_KEYS || head_dim % 16 != 0)) return NVLLM_BAD_SIZE;   // (pages)
     if ((long)num_blocks * block_size > 0x7fffffff) return NVLLM_BAD_SIZE;   // (rows of a pool are ints)
-    if (((size_t)pool_k | (size_t)pool_v) % 16 || block_pools().count(pool_k)) return NVLLM_BAD_ARGUMENT;
-    const auto known = pools().find(pool_k);
-    if (known != pools().end() && known->second.owned) return NVLLM_BAD_ARGUMENT;
+    if (((size_t)pool_k | (size_t)pool_v) % 16) return NVLLM_BAD_ARGUMENT;
     try {
+        WITH_POOLS;
+        const auto known = pools().find(pool_k);
+        if (block_pools().count(pool_k) || (known != pools().end() && known->second.owned)) return NVLLM_BAD_ARGUMENT;
         forget_shared_blocks(pool_k);
         pools()[pool_k] = PoolInfo{elem_bytes, n_layers, n_kv_heads, head_dim, false};
     } catch (const std::bad_alloc&) {
@@ -429,6 +444,7 @@ void nvllm::init_block_pool(KVCacheManager* mgr, int block_size, int num_blocks,
     mgr->pool_v = nullptr;
     BlockPool p{bytes, arrays};
     for (SlotArrays& a : p.arrays) a.base = (char*)pool + (size_t)a.base;
+    WITH_POOLS;
     block_pools()[pool] = p;
 }
 extern "C" {
@@ -436,15 +452,19 @@ extern "C" {
 void free_kv_cache_manager(KVCacheManager* mgr) {
     if (mgr->free_block_indices) free(mgr->free_block_indices);
     mgr->free_block_indices = nullptr;
-    const auto it = pools().find(mgr->pool_k);
-    const bool owned = it == pools().end() || it->second.owned;
+    bool owned = true;
     if (mgr->pool_k) {
+        WITH_POOLS;
+        const auto it = pools().find(mgr->pool_k);
+        owned = it == pools().end() || it->second.owned;
         if (it != pools().end()) pools().erase(it);
         block_pools().erase(mgr->pool_k);
         forget_shared_blocks(mgr->pool_k);
-        if (owned) device_free(mgr->pool_k);
     }
-    if (mgr->pool_v && owned) device_free(mgr->pool_v);
+    if (owned) {
+        device_free(mgr->pool_k);
+        device_free(mgr->pool_v);
+    }
     mgr->pool_k = mgr->pool_v = nullptr;
 }
 

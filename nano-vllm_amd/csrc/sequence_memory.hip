@@ -3,6 +3,8 @@
 #include "sequence_memory.h"
 
 #include <algorithm>
+#include <atomic>
+#include <mutex>
 #include <new>
 #include <numeric>
 #include <unordered_map>
@@ -276,36 +278,45 @@ int copy_slots(const std::vector<SlotArrays>& arrays, int n_slots, const int* fr
 }
 
 // ------------------------------------------------------------------ shared blocks
-// Users of a block beside its first, per pool.  A pool without forks has no entry.
+// Users of a block beside its first, per pool.  A pool without forks has no entry.  Threads that each keep a pool of their own meet in the
+// map, not in an entry, which stays where it is when others come and go.
+static std::mutex& shared_lock() {
+    static std::mutex m;
+    return m;
+}
 static std::unordered_map<const void*, std::vector<int>>& shared() {
     static std::unordered_map<const void*, std::vector<int>> m;
     return m;
 }
-static unsigned g_changes = 0;   // of the pools that have an entry
+static std::atomic<int> g_forked{0};   // entries: without one, as in programs that never fork, freeing a block takes no lock
 static std::vector<int>* users_of(const KVCacheManager* mgr) {   // null: no forks
-    static const void* pool = nullptr;   // the last one asked for: a table's blocks are freed one by one
-    static std::vector<int>* users = nullptr;
-    static unsigned seen = 0;
-    if (pool != mgr->pool_k || seen != g_changes) {
-        const auto it = shared().find(mgr->pool_k);
-        pool = mgr->pool_k;
-        users = it == shared().end() ? nullptr : &it->second;
-        seen = g_changes;
-    }
-    return users;
+    if (g_forked.load() == 0) return nullptr;
+    std::lock_guard<std::mutex> lock(shared_lock());
+    const auto it = shared().find(mgr->pool_k);
+    return it == shared().end() ? nullptr : &it->second;
 }
-static int more_users(const KVCacheManager* mgr, int block) {
-    const std::vector<int>* u = users_of(mgr);
-    return !u || block < 0 || block >= (int)u->size() ? 0 : (*u)[block];
+static std::vector<int>* make_users(const KVCacheManager* mgr) {
+    std::lock_guard<std::mutex> lock(shared_lock());
+    std::vector<int>& users = shared()[mgr->pool_k];
+    g_forked = (int)shared().size();
+    if ((int)users.size() < mgr->num_blocks) users.resize((size_t)mgr->num_blocks, 0);
+    return &users;
+}
+// users of a block beside its first, for reading and writing; null: none
+static int* more_users(const KVCacheManager* mgr, int block) {
+    std::vector<int>* u = users_of(mgr);
+    return !u || block < 0 || block >= (int)u->size() || (*u)[block] == 0 ? nullptr : &(*u)[block];
 }
 bool drop_shared_block(const KVCacheManager* mgr, int block) {
-    if (more_users(mgr, block) == 0) return false;
-    (*users_of(mgr))[block]--;
+    int* more = more_users(mgr, block);
+    if (!more) return false;
+    (*more)--;
     return true;
 }
 void forget_shared_blocks(const void* pool_k) {
+    std::lock_guard<std::mutex> lock(shared_lock());
     shared().erase(pool_k);
-    g_changes++;
+    g_forked = (int)shared().size();
 }
 
 // which blocks lie on the free stack; empty: the stack is not one of this pool
@@ -379,14 +390,7 @@ int nvllm_fork_tables(KVCacheManager* mgr, const BlockTable* from, int positions
             for (int i = 0; i < n; i++) target.push_back(mgr->free_block_indices[mgr->free_blocks_count - 1 - i]);
         }
         std::vector<int>* users = nullptr;
-        if (whole > 0) {
-            users = users_of(mgr);
-            if (!users) {
-                users = &shared()[mgr->pool_k];
-                g_changes++;
-            }
-            if ((int)users->size() < mgr->num_blocks) users->resize((size_t)mgr->num_blocks, 0);
-        }
+        if (whole > 0) users = make_users(mgr);
         if (tail)
             if (const int e = copy_slots(arrays, mgr->num_blocks, source.data(), target.data(), n)) return e;
         // (nothing below fails)
@@ -403,7 +407,8 @@ int nvllm_block_users(const KVCacheManager* mgr, int block) {
     if (!usable(mgr) || block < 0 || block >= mgr->num_blocks) return NVLLM_BAD_ARGUMENT;
     for (int i = 0; i < mgr->free_blocks_count; i++)
         if (mgr->free_block_indices[i] == block) return 0;
-    return 1 + more_users(mgr, block);
+    const int* more = more_users(mgr, block);
+    return 1 + (more ? *more : 0);
 }
 
 int nvllm_free_table(KVCacheManager* mgr, BlockTable* table) {
@@ -435,11 +440,13 @@ int nvllm_compact_blocks(KVCacheManager* mgr, BlockTable** tables, int n) {
             }
         }
         const int used = mgr->num_blocks - mgr->free_blocks_count;
+        std::vector<int>* users = users_of(mgr);
+        if (users && (int)users->size() < mgr->num_blocks) users->resize((size_t)mgr->num_blocks, 0);
         std::vector<int> from, to, place((size_t)mgr->num_blocks);
         std::iota(place.begin(), place.end(), 0);
         int hole = 0;
         for (int b = used; b < mgr->num_blocks; b++) {
-            if (is_free[b] || found[b] == 0 || found[b] < 1 + more_users(mgr, b)) continue;
+            if (is_free[b] || found[b] == 0 || (users && found[b] < 1 + (*users)[b])) continue;
             while (!is_free[hole]) hole++;   // (there are as many below `used` as blocks in use behind it)
             from.push_back(b);
             to.push_back(hole);
@@ -448,7 +455,6 @@ int nvllm_compact_blocks(KVCacheManager* mgr, BlockTable** tables, int n) {
         if (!from.empty())
             if (const int e = copy_slots(arrays, mgr->num_blocks, from.data(), to.data(), (int)from.size())) return e;
         // (nothing below fails)
-        std::vector<int>* users = users_of(mgr);
         for (size_t i = 0; i < from.size(); i++) {
             is_free[from[i]] = 1;
             is_free[to[i]] = 0;
