@@ -7,6 +7,7 @@
 #include <mutex>
 #include <new>
 #include <unordered_map>
+#include <unordered_set>
 #include <vector>
 
 #include "gemm_f32.h"
@@ -30,7 +31,8 @@ static std::mutex& pools_lock() {
 struct PoolInfo {
     int elem_bytes;
     int n_layers, n_kv_heads, head_dim;
-    bool owned;   // by the library: free_kv_cache_manager frees the memory
+    bool owned;         // by the library
+    const int* stack;   // the free stack of the manager that has it
 };
 // Block pools of models that lay them out themselves: bytes behind pool_k, and where the blocks lie.
 struct BlockPool {
@@ -51,6 +53,11 @@ static std::unordered_map<const void*, PoolInfo>& pools() {
     static std::unordered_map<const void*, PoolInfo> m;
     return m;
 }
+// Managers (by their free stacks, which are their own) whose memory is the caller's to free, whatever became of it since.
+static std::unordered_set<const int*>& attached() {
+    static std::unordered_set<const int*> s;
+    return s;
+}
 
 std::vector<SlotArrays> pool_arrays(const KVCacheManager* mgr) {
     WITH_POOLS;
@@ -59,6 +66,7 @@ std::vector<SlotArrays> pool_arrays(const KVCacheManager* mgr) {
     const auto it = pools().find(mgr->pool_k);
     if (it == pools().end()) return {};
     const PoolInfo& p = it->second;
+    if (!p.owned && p.stack != mgr->free_block_indices) return {};   // (attached again: a later manager's)
     const size_t block = (size_t)mgr->block_size * p.n_kv_heads * p.head_dim * p.elem_bytes;
     return {SlotArrays{mgr->pool_k, block, block * mgr->num_blocks, p.n_layers}, SlotArrays{mgr->pool_v, block, block * mgr->num_blocks, p.n_layers}};
 }
@@ -378,6 +386,9 @@ static void init_free_stack(KVCacheManager* mgr, int block_size, int num_blocks)
     mgr->free_blocks_count = num_blocks;
     mgr->free_block_indices = (int*)malloc((size_t)num_blocks * sizeof(int));
     for (int slot = 0; slot < num_blocks; slot++) mgr->free_block_indices[slot] = num_blocks - 1 - slot;
+    WITH_POOLS;   // (what is known of a manager whose stack lay here)
+    attached().erase(mgr->free_block_indices);
+    forget_shared_blocks(mgr->free_block_indices);
 }
 
 void init_kv_cache_manager(KVCacheManager* mgr, int block_size, int num_blocks, int n_layers,
@@ -409,7 +420,7 @@ void init_kv_cache_manager(KVCacheManager* mgr, int block_size, int num_blocks, 
     mgr->pool_k = (float*)pk;
     mgr->pool_v = (float*)pv;
     WITH_POOLS;
-    pools()[pk] = PoolInfo{eb, n_layers, n_kv_heads, head_dim, true};
+    pools()[pk] = PoolInfo{eb, n_layers, n_kv_heads, head_dim, true, mgr->free_block_indices};
 }
 
 int nvllm_attach_kv_pool(KVCacheManager* mgr, int block_size, int num_blocks, int n_layers, int n_kv_heads, int head_dim, int elem_bytes, void* pool_k, void* pool_v) {
@@ -418,19 +429,25 @@ int nvllm_attach_kv_pool(KVCacheManager* mgr, int block_size, int num_blocks, in
     if (elem_bytes == 2 && (block_size != KV16_PAGE_KEYS || head_dim % 16 != 0)) return NVLLM_BAD_SIZE;   // (pages)
     if ((long)num_blocks * block_size > 0x7fffffff) return NVLLM_BAD_SIZE;   // (rows of a pool are ints)
     if (((size_t)pool_k | (size_t)pool_v) % 16) return NVLLM_BAD_ARGUMENT;
+    KVCacheManager m = *mgr;
+    init_free_stack(&m, block_size, num_blocks);
+    m.pool_k = (float*)pool_k;
+    m.pool_v = (float*)pool_v;
+    int refusal = 0;
     try {
         WITH_POOLS;
         const auto known = pools().find(pool_k);
-        if (block_pools().count(pool_k) || (known != pools().end() && known->second.owned)) return NVLLM_BAD_ARGUMENT;
-        forget_shared_blocks(pool_k);
-        pools()[pool_k] = PoolInfo{elem_bytes, n_layers, n_kv_heads, head_dim, false};
+        if (block_pools().count(pool_k) || (known != pools().end() && known->second.owned)) refusal = NVLLM_BAD_ARGUMENT;
+        else {
+            attached().insert(m.free_block_indices);
+            pools()[pool_k] = PoolInfo{elem_bytes, n_layers, n_kv_heads, head_dim, false, m.free_block_indices};
+        }
     } catch (const std::bad_alloc&) {
-        return NVLLM_NO_MEMORY;
+        refusal = NVLLM_NO_MEMORY;
     }
-    init_free_stack(mgr, block_size, num_blocks);
-    mgr->pool_k = (float*)pool_k;
-    mgr->pool_v = (float*)pool_v;
-    return 0;
+    if (refusal == 0) *mgr = m;
+    else free(m.free_block_indices);
+    return refusal;
 }
 
 }  // extern "C"
@@ -445,22 +462,24 @@ void nvllm::init_block_pool(KVCacheManager* mgr, int block_size, int num_blocks,
     BlockPool p{bytes, arrays};
     for (SlotArrays& a : p.arrays) a.base = (char*)pool + (size_t)a.base;
     WITH_POOLS;
+    pools().erase(pool);   // (what was attached there is gone)
     block_pools()[pool] = p;
 }
 extern "C" {
 
 void free_kv_cache_manager(KVCacheManager* mgr) {
+    bool owned = true;
+    {
+        WITH_POOLS;
+        const int* stack = mgr->free_block_indices;
+        const auto it = pools().find(mgr->pool_k);
+        owned = attached().erase(stack) == 0 && (it == pools().end() || it->second.owned);
+        if (it != pools().end() && (owned || it->second.stack == stack)) pools().erase(it);
+        if (owned) block_pools().erase(mgr->pool_k);
+        forget_shared_blocks(stack);
+    }
     if (mgr->free_block_indices) free(mgr->free_block_indices);
     mgr->free_block_indices = nullptr;
-    bool owned = true;
-    if (mgr->pool_k) {
-        WITH_POOLS;
-        const auto it = pools().find(mgr->pool_k);
-        owned = it == pools().end() || it->second.owned;
-        if (it != pools().end()) pools().erase(it);
-        block_pools().erase(mgr->pool_k);
-        forget_shared_blocks(mgr->pool_k);
-    }
     if (owned) {
         device_free(mgr->pool_k);
         device_free(mgr->pool_v);

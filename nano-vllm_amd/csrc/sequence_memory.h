@@ -19,11 +19,11 @@ struct SlotArrays {
 // (nothing is enqueued then).
 int copy_slots(const std::vector<SlotArrays>& arrays, int n_slots, const int* from, const int* to, int n);
 
-// ops_api.hip: the arrays of a pool's blocks; empty: not a pool of this library
+// ops_api.hip: the arrays of a pool's blocks; empty: not a pool of this library, or memory that a later manager has
 std::vector<SlotArrays> pool_arrays(const KVCacheManager* mgr);
 // sequence_memory.hip: one of a shared block's users lets go of it; false: it has one user only
 bool drop_shared_block(const KVCacheManager* mgr, int block);
-void forget_shared_blocks(const void* pool_k);   // the pool is gone
+void forget_shared_blocks(const int* stack);   // the manager with this free stack is gone
 
 // Is the library stream being captured?  (Entry points whose arguments are host arrays refuse that: a replay would read what the
 // arrays' staging holds by then.)

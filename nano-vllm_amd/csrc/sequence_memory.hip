@@ -278,26 +278,26 @@ int copy_slots(const std::vector<SlotArrays>& arrays, int n_slots, const int* fr
 }
 
 // ------------------------------------------------------------------ shared blocks
-// Users of a block beside its first, per pool.  A pool without forks has no entry.  Threads that each keep a pool of their own meet in the
+// Users of a block beside its first, per manager (by its free stack, which no other has).  Without forks there is no entry.  Threads that each keep a pool of their own meet in the
 // map, not in an entry, which stays where it is when others come and go.
 static std::mutex& shared_lock() {
     static std::mutex m;
     return m;
 }
-static std::unordered_map<const void*, std::vector<int>>& shared() {
-    static std::unordered_map<const void*, std::vector<int>> m;
+static std::unordered_map<const int*, std::vector<int>>& shared() {
+    static std::unordered_map<const int*, std::vector<int>> m;
     return m;
 }
 static std::atomic<int> g_forked{0};   // entries: without one, as in programs that never fork, freeing a block takes no lock
 static std::vector<int>* users_of(const KVCacheManager* mgr) {   // null: no forks
     if (g_forked.load() == 0) return nullptr;
     std::lock_guard<std::mutex> lock(shared_lock());
-    const auto it = shared().find(mgr->pool_k);
+    const auto it = shared().find(mgr->free_block_indices);
     return it == shared().end() ? nullptr : &it->second;
 }
 static std::vector<int>* make_users(const KVCacheManager* mgr) {
     std::lock_guard<std::mutex> lock(shared_lock());
-    std::vector<int>& users = shared()[mgr->pool_k];
+    std::vector<int>& users = shared()[mgr->free_block_indices];
     g_forked = (int)shared().size();
     if ((int)users.size() < mgr->num_blocks) users.resize((size_t)mgr->num_blocks, 0);
     return &users;
@@ -313,9 +313,9 @@ bool drop_shared_block(const KVCacheManager* mgr, int block) {
     (*more)--;
     return true;
 }
-void forget_shared_blocks(const void* pool_k) {
+void forget_shared_blocks(const int* stack) {
     std::lock_guard<std::mutex> lock(shared_lock());
-    shared().erase(pool_k);
+    shared().erase(stack);
     g_forked = (int)shared().size();
 }
 
