@@ -189,7 +189,8 @@ int nvllm_copy_blocks(KVCacheManager* mgr, const int* from, const int* to, int n
 int nvllm_fork_tables(KVCacheManager* mgr, const BlockTable* from, int positions, BlockTable** to, int n);
 /* Tables that have the block (0: it is free), as far as nvllm_fork_tables made them; or a refusal. */
 int nvllm_block_users(const KVCacheManager* mgr, int block);
-/* free_block() on every block of a table, the last one first; the table is empty then. */
+/* free_block() on every block of a table, the last one first; the table is empty then.  NVLLM_BAD_INDEX, and nothing is freed, for a table
+ * that names a block twice or one that is free. */
 int nvllm_free_table(KVCacheManager* mgr, BlockTable* table);
 
 /* Moves blocks in use to the lowest numbers, in the order of theirs, and writes the given tables anew; the free blocks are then

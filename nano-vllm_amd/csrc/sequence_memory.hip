@@ -330,6 +330,32 @@ static std::vector<char> free_blocks(const KVCacheManager* mgr) {
     }
     return is_free;
 }
+// A table's release: how many blocks go back to the pool; a refusal for a table that names a block twice, or one that is free.  A shared block is
+// in use; the free stack, which the caller may write too, is read for the others: 0.2 us for 512 free blocks, 3 for 8,192.
+static int blocks_to_free(const KVCacheManager* mgr, const BlockTable* table, const std::vector<int>* users) {
+    const unsigned n = (unsigned)mgr->num_blocks;
+    static thread_local std::vector<unsigned char> marks;   // all zeros between calls
+    if (marks.size() < (size_t)n + 1) marks.resize((size_t)n + 1, 0);
+    unsigned char* mark = marks.data();
+    auto shared = [&](unsigned b) { return users && b < users->size() && (*users)[b] > 0; };
+    int met = 0, back = 0;
+    for (; met < table->num_blocks; met++) {
+        const unsigned b = (unsigned)table->block_indices[met];
+        if (b >= n || mark[b]) break;
+        mark[b] = shared(b) ? 1 : 2;
+        back += mark[b] - 1;
+    }
+    bool fits = met == table->num_blocks && mgr->free_blocks_count >= 0 && mgr->free_blocks_count <= mgr->num_blocks - back;
+    if (fits && back > 0) {
+        mark[n] = 2;   // (what is no block of the pool)
+        unsigned char any = 0;
+        for (int i = 0; i < mgr->free_blocks_count; i++) any |= mark[std::min((unsigned)mgr->free_block_indices[i], n)];
+        mark[n] = 0;
+        fits = any < 2;
+    }
+    while (met-- > 0) mark[table->block_indices[met]] = 0;
+    return fits ? back : NVLLM_BAD_INDEX;
+}
 static bool usable(const KVCacheManager* mgr) { return mgr && mgr->free_block_indices && mgr->num_blocks > 0 && mgr->block_size > 0; }
 
 }  // namespace nvllm
@@ -413,10 +439,17 @@ int nvllm_block_users(const KVCacheManager* mgr, int block) {
 
 int nvllm_free_table(KVCacheManager* mgr, BlockTable* table) {
     if (!usable(mgr) || !table || table->num_blocks < 0 || (table->num_blocks > 0 && !table->block_indices)) return NVLLM_BAD_ARGUMENT;
-    for (int i = 0; i < table->num_blocks; i++)
-        if (table->block_indices[i] < 0 || table->block_indices[i] >= mgr->num_blocks) return NVLLM_BAD_INDEX;
-    for (; table->num_blocks > 0; table->num_blocks--) free_block(mgr, table->block_indices[table->num_blocks - 1]);
-    return 0;
+    if (table->num_blocks == 0) return 0;
+    REFUSING(
+        std::vector<int>* users = users_of(mgr);
+        const int back = blocks_to_free(mgr, table, users);
+        if (back < 0) return back;
+        for (; table->num_blocks > 0; table->num_blocks--) {
+            const int b = table->block_indices[table->num_blocks - 1];
+            if (users && b < (int)users->size() && (*users)[b] > 0) (*users)[b]--;
+            else mgr->free_block_indices[mgr->free_blocks_count++] = b;
+        }
+        return 0;)
 }
 
 int nvllm_compact_blocks(KVCacheManager* mgr, BlockTable** tables, int n) {
