@@ -461,6 +461,7 @@ int nvllm_compact_blocks(KVCacheManager* mgr, BlockTable** tables, int n) {
         if (is_free.empty()) return NVLLM_BAD_INDEX;
         // how many of the given tables have a block: one that others use too stays where it is, like one that no table has
         std::vector<int> found((size_t)mgr->num_blocks, 0);
+        std::vector<const BlockTable*> last((size_t)mgr->num_blocks, nullptr);   // (a table that names a block twice is one)
         std::vector<BlockTable*> all(tables, tables + n);
         std::sort(all.begin(), all.end());
         if (std::adjacent_find(all.begin(), all.end()) != all.end()) return NVLLM_BAD_ARGUMENT;
@@ -469,7 +470,8 @@ int nvllm_compact_blocks(KVCacheManager* mgr, BlockTable** tables, int n) {
             for (int i = 0; i < t->num_blocks; i++) {
                 const int b = t->block_indices[i];
                 if (b < 0 || b >= mgr->num_blocks || is_free[b]) return NVLLM_BAD_INDEX;
-                found[b]++;
+                found[b] += last[b] != t;
+                last[b] = t;
             }
         }
         const int used = mgr->num_blocks - mgr->free_blocks_count;
