@@ -1227,17 +1227,59 @@ static int chunk_min(const Delta& a, const std::vector<int4>& spans, bool b16) {
 // the other; n segments of m chunks take about m / n + DC n / 2.5 of a chunk's time, least at sqrt(2.5 m / DC).  Measured, in one segment and
 // in this many: 8,192 tokens, one head of 128 x 128: 194 us, 83 in 8; four: 195, 105 in 5; eight: 201, 146 in 3 (161 in 4, which no longer
 // fit side by side); one of 64 x 64: 174, 58 in 12; 4,096 tokens, two of 256 x 256: 157, 117 in 4; 1,024 tokens, one of 128 x 128: 35, 39 in 3.
-static void delta_segments(DeltaChunks& c, int DC, int most) {
-    const Delta& a = c.a;
-    const long walks = (long)a.H * cdiv(a.vdim, 16) * a.n_spans, unit = (long)a.H * 2 * DC * a.n_spans, cus = rt().num_cus;
-    c.segs = 1;
-    c.per_seg = most;
+static void delta_segments(const Delta& a, int n_spans, int DC, int most, int& segs, int& per_seg) {
+    const long walks = (long)a.H * cdiv(a.vdim, 16) * n_spans, unit = (long)a.H * 2 * DC * n_spans, cus = rt().num_cus;
+    segs = 1;
+    per_seg = most;
     if (most < 6 * DC || walks + unit > cus) return;
     const long fit = std::min(2 + (cus - walks) / (walks + unit), cus / walks), best = (long)sqrt(2.5 * most / DC);
-    const int segs = (int)std::min(fit, best);
-    if (segs < 3) return;
-    c.per_seg = cdiv(most, segs);
-    c.segs = cdiv(most, c.per_seg);
+    const int n = (int)std::min(fit, best);
+    if (n < 3) return;
+    per_seg = cdiv(most, n);
+    segs = cdiv(most, per_seg);
+}
+
+// Portions whose chunks are prepared and walked together, `most` chunks of each per launch: as many portions as have room for the records of one
+// chunk each, and then as many chunks.
+struct DeltaGroup {
+    int at, n, most, longest, segs, per_seg;
+    long tokens;
+    double states;                         // bytes
+    size_t records, start_floats, bytes;   // of a launch
+};
+static std::vector<DeltaGroup> delta_groups(const Delta& a, const std::vector<int4>& spans, int n_chunked, std::vector<int>& first) {
+    const size_t room = std::max((size_t)1, CHUNK_MEMORY / ((size_t)a.H * DELTA_RECORD));
+    const int steps = cdiv(a.dim, 32), DC = steps <= 4 ? steps : steps <= 6 ? 6 : 8;
+    const int n_groups = (int)((n_chunked + room - 1) / room), portions = n_groups ? cdiv(n_chunked, n_groups) : 0;   // of one size, or about
+    std::vector<DeltaGroup> groups;
+    for (int at = 0; at < n_chunked;) {
+        DeltaGroup g{};
+        g.at = at;
+        g.n = std::min(n_chunked - at, portions);
+        for (int i = at; i < at + g.n; i++) {
+            g.tokens += spans[i].y;
+            g.states += (spans[i].z > 0 ? 8.0 : 4.0) * a.H * a.dim * (double)a.vdim;
+            g.longest = std::max(g.longest, cdiv(spans[i].y, CH));
+        }
+        auto records = [&](int per) {
+            size_t n = 0;
+            for (int i = at; i < at + g.n; i++) {
+                first[i] = (int)n;
+                n += (size_t)std::min(per, cdiv(spans[i].y, CH));
+            }
+            return n;
+        };
+        g.most = g.longest;
+        while (g.most > 1 && records(g.most) > room) g.most = (g.most + 1) / 2;
+        g.records = records(g.most);
+        delta_segments(a, g.n, DC, g.most, g.segs, g.per_seg);
+        const size_t columns = (size_t)((a.vdim + 15) & ~15), places = g.segs > 1 ? (size_t)g.n * g.segs * a.H * (32 * DC) : 0;
+        g.start_floats = places * columns;
+        g.bytes = g.records * a.H * DELTA_RECORD + places * (columns + 32 * DC) * sizeof(float);
+        groups.push_back(g);
+        at += g.n;
+    }
+    return groups;
 }
 
 static int gated_delta(Delta& a, const int* seq_ids, const int* pos, int T, int n_slots, int elem) {
@@ -1247,39 +1289,18 @@ static int gated_delta(Delta& a, const int* seq_ids, const int* pos, int T, int 
     const bool b16 = elem == 2;
     const int least = chunk_min(a, spans, b16);   // portions that go by chunks come first
     std::stable_sort(spans.begin(), spans.end(), [&](const int4& l, const int4& r) { return (l.y >= least) > (r.y >= least); });
-    int n_chunked = 0, longest = 0;
-    long tokens = 0;
-    double states[2] = {0, 0};
+    int n_chunked = 0;
+    double tok_states = 0;
     for (const int4& s : spans) {
-        const bool ch = s.y >= least;
-        states[ch] += (s.z > 0 ? 8.0 : 4.0) * a.H * a.dim * (double)a.vdim;
-        if (!ch) continue;
-        n_chunked++;
-        tokens += s.y;
-        longest = std::max(longest, cdiv(s.y, CH));
-    }
-    // chunks of every portion per launch, and each portion's first record then
-    int most = 0;
-    std::vector<int> first(spans.size(), 0);
-    if (n_chunked > 0) {
-        const size_t room = std::max((size_t)1, CHUNK_MEMORY / ((size_t)a.H * DELTA_RECORD));
-        auto records = [&](int per) {
-            size_t n = 0;
-            for (int i = 0; i < n_chunked; i++) {
-                first[i] = (int)n;
-                n += (size_t)std::min(per, cdiv(spans[i].y, CH));
-            }
-            return n;
-        };
-        most = longest;
-        while (most > 1 && records(most) > room) most = (most + 1) / 2;
-        (void)records(most);
-        if (n_chunked > 65535 || most > 65535) return NVLLM_BAD_SIZE;
+        if (s.y >= least) n_chunked++;
+        else tok_states += (s.z > 0 ? 8.0 : 4.0) * a.H * a.dim * (double)a.vdim;
     }
     const size_t ints = spans.size() * 5 + 4;
     if (ints > staging_ints()) return NVLLM_BAD_SIZE;
     ensure_init();
     if (stream_is_captured()) return NVLLM_CAPTURED;
+    std::vector<int> first(spans.size(), 0);
+    const std::vector<DeltaGroup> groups = delta_groups(a, spans, n_chunked, first);
     const int4* d_spans = nullptr;
     const int* d_first = nullptr;
     if (spans.size() > DELTA_SPANS) {
@@ -1296,28 +1317,20 @@ static int gated_delta(Delta& a, const int* seq_ids, const int* pos, int T, int 
                      (size_t)a.v % four == 0 && (size_t)a.out % four == 0 && (size_t)a.state % 16 == 0;
     a.n_spans = (int)spans.size() - n_chunked;
     const double token_bytes = elem * (2.0 * a.Q * a.dim + 2.0 * a.H * a.vdim) + 8.0 * a.H, token_flops = 6.0 * a.H * a.dim * (double)a.vdim;
+    long tokens = 0;
+    for (const DeltaGroup& gr : groups) tokens += gr.tokens;
     if (n_chunked > 0) {
         DeltaChunks c{};
         c.a = a;
-        c.a.n_spans = n_chunked;
-        c.a.spans = d_spans;
-        c.first = d_first;
-        if (!d_spans) {
-            std::copy(spans.begin(), spans.end(), c.a.here);
-            std::copy(first.begin(), first.begin() + n_chunked, c.first_here);
-        }
         c.out_four = a.vdim % 4 == 0 && (size_t)a.out % (4 * elem) == 0;
-        size_t n_records = 0;
-        for (int i = 0; i < n_chunked; i++) n_records = std::max(n_records, (size_t)first[i] + std::min(most, cdiv(spans[i].y, CH)));
-        const int steps = cdiv(a.dim, 32), DC = steps <= 4 ? steps : steps <= 6 ? 6 : 8;
-        delta_segments(c, DC, most);
-        const size_t columns = (size_t)((a.vdim + 15) & ~15), places = c.segs > 1 ? (size_t)n_chunked * c.segs * a.H * (32 * DC) : 0;
         const int per16 = 16 / elem, dim_ld = (a.dim + 7) & ~7, vdim_ld = (a.vdim + 7) & ~7;
         const bool fits = a.dim % 8 == 0 && a.q_ld % per16 == 0 && a.k_ld % per16 == 0 && ((size_t)a.q | (size_t)a.k) % 16 == 0;
         const bool v_fits = a.vdim % per16 == 0 && a.v_ld % per16 == 0 && (size_t)a.v % 16 == 0;
         auto room = [&](bool needed, int heads, int ld) { return needed ? ((size_t)T * heads * ld * elem + 255) & ~(size_t)255 : 0; };
         const size_t qk_room = room(!fits, a.Q, dim_ld), v_room = room(!v_fits, a.H, vdim_ld);
-        char* mem = (char*)ws_get(WS_DELTA, 2 * qk_room + v_room + n_records * a.H * DELTA_RECORD + places * (columns + 32 * DC) * sizeof(float));
+        size_t most_bytes = 0;
+        for (const DeltaGroup& gr : groups) most_bytes = std::max(most_bytes, gr.bytes);
+        char* mem = (char*)ws_get(WS_DELTA, 2 * qk_room + v_room + most_bytes);
         auto pack = [&](const void*& src, long& ld, int heads, int dim, int wide) {
             if (b16) NVLLM_LAUNCH((k_delta_rows<unsigned short>), dim3(T), dim3(256), 0, (unsigned short*)mem, (const unsigned short*)src, heads, dim, wide, ld);
             else NVLLM_LAUNCH((k_delta_rows<float>), dim3(T), dim3(256), 0, (float*)mem, (const float*)src, heads, dim, wide, ld);
@@ -1338,33 +1351,44 @@ static int gated_delta(Delta& a, const int* seq_ids, const int* pos, int T, int 
             c.a.v_cols = vdim_ld;
         }
         c.mem = mem;
-        c.starts = (float*)(mem + n_records * a.H * DELTA_RECORD);
-        c.trans = c.starts + places * columns;
-        // the algorithm's bytes and flops, split over the launches
-        const int rounds = cdiv(longest, most);
-        c.bytes = (states[1] + (double)tokens * token_bytes) / rounds;
-        c.flops = (double)tokens * token_flops / rounds;
-        // The others' steps go with the first chunks' launch where rows are aligned for both.  Apart and together: three portions of 512 tokens
-        // and eleven of one, 32 heads of 64 x 64: 36.5 us, 32.0; one of 512 and 64, 128 x 128: 83, 72 (in 32 bits 101, 89); four of 1,024
-        // and 64: 207, 199 (350, 340).
-        const long waves = (long)cdiv(a.vdim, STEP_COLS) * a.H * ((long)spans.size() - n_chunked);
-        if (fits && v_fits && vec && n_chunked + waves / (4L * a.H * most) < 65535) {
-            c.step_waves = (int)waves;
-            c.bytes += (states[0] + (double)(T - tokens) * token_bytes) / rounds;
-            c.flops += (double)(T - tokens) * token_flops / rounds;
-            a.n_spans = 0;
-        }
-        for (c.from = 0; c.from < longest; c.from += most) {
-            c.most = std::min(most, longest - c.from);
-            if (b16) launch_chunks<true>(c);
-            else launch_chunks<false>(c);
-            c.step_waves = 0;
+        for (const DeltaGroup& gr : groups) {
+            c.a.n_spans = gr.n;
+            c.a.spans = d_spans ? d_spans + gr.at : nullptr;
+            c.first = d_first ? d_first + gr.at : nullptr;
+            if (!d_spans) {
+                std::copy(spans.begin() + gr.at, spans.end(), c.a.here);
+                std::copy(first.begin() + gr.at, first.begin() + gr.at + gr.n, c.first_here);
+            }
+            c.segs = gr.segs;
+            c.per_seg = gr.per_seg;
+            c.starts = (float*)(mem + gr.records * a.H * DELTA_RECORD);
+            c.trans = c.starts + gr.start_floats;
+            // the algorithm's bytes and flops, split over the launches
+            const int rounds = cdiv(gr.longest, gr.most);
+            c.bytes = (gr.states + (double)gr.tokens * token_bytes) / rounds;
+            c.flops = (double)gr.tokens * token_flops / rounds;
+            // The others' steps go with the last group's first launch where rows are aligned for both.  Apart and together: three portions of 512 tokens
+            // and eleven of one, 32 heads of 64 x 64: 36.5 us, 32.0; one of 512 and 64, 128 x 128: 83, 72 (in 32 bits 101, 89); four of 1,024
+            // and 64: 207, 199 (350, 340).
+            const long waves = (long)cdiv(a.vdim, STEP_COLS) * a.H * a.n_spans;
+            if (gr.at + gr.n == n_chunked && fits && v_fits && vec && gr.n + waves / (4L * a.H * gr.most) < 65535) {
+                c.step_waves = (int)waves;
+                c.bytes += (tok_states + (double)(T - tokens) * token_bytes) / rounds;
+                c.flops += (double)(T - tokens) * token_flops / rounds;
+                a.n_spans = 0;
+            }
+            for (c.from = 0; c.from < gr.longest; c.from += gr.most) {
+                c.most = std::min(gr.most, gr.longest - c.from);
+                if (b16) launch_chunks<true>(c);
+                else launch_chunks<false>(c);
+                c.step_waves = 0;
+            }
         }
     }
     if (a.n_spans == 0) return 0;
     a.spans = d_spans ? d_spans + n_chunked : nullptr;
     if (!d_spans) std::copy(spans.begin() + n_chunked, spans.end(), a.here);
-    ProfScope ps(PC_DELTA_TOK, states[0] + (double)(T - tokens) * token_bytes, (double)(T - tokens) * token_flops);
+    ProfScope ps(PC_DELTA_TOK, tok_states + (double)(T - tokens) * token_bytes, (double)(T - tokens) * token_flops);
     for (int left = a.n_spans; left > 0; left -= a.n_spans, a.spans += a.n_spans) {   // (what a grid takes)
         a.n_spans = std::min(left, 65535);
         if (b16 && vec) launch_step<true, true>(a);
