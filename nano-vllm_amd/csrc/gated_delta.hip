@@ -1301,17 +1301,6 @@ static int gated_delta(Delta& a, const int* seq_ids, const int* pos, int T, int 
     if (stream_is_captured()) return NVLLM_CAPTURED;
     std::vector<int> first(spans.size(), 0);
     const std::vector<DeltaGroup> groups = delta_groups(a, spans, n_chunked, first);
-    const int4* d_spans = nullptr;
-    const int* d_first = nullptr;
-    if (spans.size() > DELTA_SPANS) {
-        int* host = pinned_ints(ints);
-        std::copy(spans.begin(), spans.end(), (int4*)host);
-        std::copy(first.begin(), first.end(), host + 4 * spans.size());
-        int* dev = (int*)ws_get(WS_STEP, ints * sizeof(int));
-        launch_copy_ints(dev, host, spans.size() * 5);
-        d_spans = (const int4*)dev;
-        d_first = dev + 4 * spans.size();
-    }
     const size_t four = 4 * (size_t)elem;
     const bool vec = a.dim % 4 == 0 && a.vdim % 4 == 0 && a.q_ld % 4 == 0 && a.k_ld % 4 == 0 && a.v_ld % 4 == 0 && (size_t)a.q % four == 0 && (size_t)a.k % four == 0 &&
                      (size_t)a.v % four == 0 && (size_t)a.out % four == 0 && (size_t)a.state % 16 == 0;
@@ -1319,18 +1308,32 @@ static int gated_delta(Delta& a, const int* seq_ids, const int* pos, int T, int 
     const double token_bytes = elem * (2.0 * a.Q * a.dim + 2.0 * a.H * a.vdim) + 8.0 * a.H, token_flops = 6.0 * a.H * a.dim * (double)a.vdim;
     long tokens = 0;
     for (const DeltaGroup& gr : groups) tokens += gr.tokens;
+    const int per16 = 16 / elem, dim_ld = (a.dim + 7) & ~7, vdim_ld = (a.vdim + 7) & ~7;
+    const bool fits = a.dim % 8 == 0 && a.q_ld % per16 == 0 && a.k_ld % per16 == 0 && ((size_t)a.q | (size_t)a.k) % 16 == 0;
+    const bool v_fits = a.vdim % per16 == 0 && a.v_ld % per16 == 0 && (size_t)a.v % 16 == 0;
+    auto room = [&](bool needed, int heads, int ld) { return needed ? ((size_t)T * heads * ld * elem + 255) & ~(size_t)255 : 0; };
+    const size_t qk_room = room(!fits, a.Q, dim_ld), v_room = room(!v_fits, a.H, vdim_ld);
+    size_t most_bytes = 0;
+    for (const DeltaGroup& gr : groups) most_bytes = std::max(most_bytes, gr.bytes);
+    // (all of the memory before the first launch)
+    const size_t rows_bytes = n_chunked > 0 ? 2 * qk_room + v_room + most_bytes : 0, step_bytes = spans.size() > DELTA_SPANS ? ints * sizeof(int) : 0;
+    char* mem = (char*)ws_try(WS_DELTA, rows_bytes);
+    int* dev = (int*)ws_try(WS_STEP, step_bytes);
+    if ((rows_bytes > 0 && !mem) || (step_bytes > 0 && !dev)) return NVLLM_NO_MEMORY;
+    const int4* d_spans = nullptr;
+    const int* d_first = nullptr;
+    if (spans.size() > DELTA_SPANS) {
+        int* host = pinned_ints(ints);
+        std::copy(spans.begin(), spans.end(), (int4*)host);
+        std::copy(first.begin(), first.end(), host + 4 * spans.size());
+        launch_copy_ints(dev, host, spans.size() * 5);
+        d_spans = (const int4*)dev;
+        d_first = dev + 4 * spans.size();
+    }
     if (n_chunked > 0) {
         DeltaChunks c{};
         c.a = a;
         c.out_four = a.vdim % 4 == 0 && (size_t)a.out % (4 * elem) == 0;
-        const int per16 = 16 / elem, dim_ld = (a.dim + 7) & ~7, vdim_ld = (a.vdim + 7) & ~7;
-        const bool fits = a.dim % 8 == 0 && a.q_ld % per16 == 0 && a.k_ld % per16 == 0 && ((size_t)a.q | (size_t)a.k) % 16 == 0;
-        const bool v_fits = a.vdim % per16 == 0 && a.v_ld % per16 == 0 && (size_t)a.v % 16 == 0;
-        auto room = [&](bool needed, int heads, int ld) { return needed ? ((size_t)T * heads * ld * elem + 255) & ~(size_t)255 : 0; };
-        const size_t qk_room = room(!fits, a.Q, dim_ld), v_room = room(!v_fits, a.H, vdim_ld);
-        size_t most_bytes = 0;
-        for (const DeltaGroup& gr : groups) most_bytes = std::max(most_bytes, gr.bytes);
-        char* mem = (char*)ws_get(WS_DELTA, 2 * qk_room + v_room + most_bytes);
         auto pack = [&](const void*& src, long& ld, int heads, int dim, int wide) {
             if (b16) NVLLM_LAUNCH((k_delta_rows<unsigned short>), dim3(T), dim3(256), 0, (unsigned short*)mem, (const unsigned short*)src, heads, dim, wide, ld);
             else NVLLM_LAUNCH((k_delta_rows<float>), dim3(T), dim3(256), 0, (float*)mem, (const float*)src, heads, dim, wide, ld);
