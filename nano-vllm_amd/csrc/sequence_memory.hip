@@ -247,11 +247,12 @@ int copy_slots(const std::vector<SlotArrays>& arrays, int n_slots, const int* fr
     CopyArgs a{};
     a.n_programs = plan.programs();
     const bool here = ints <= COPY_INLINE;
+    int* dev = here ? nullptr : (int*)ws_try(WS_STEP, (ints + 4) * sizeof(int));
+    if (!here && !dev) return NVLLM_NO_MEMORY;
     int* host = here ? a.here : pinned_ints((ints + 3) & ~(size_t)3);
     std::copy(plan.first.begin(), plan.first.end(), host);
     std::copy(plan.moves.begin(), plan.moves.end(), host + plan.first.size());
     if (!here) {
-        int* dev = (int*)ws_get(WS_STEP, (ints + 4) * sizeof(int));
         launch_copy_ints(dev, host, ints);
         a.programs = dev;
     }
