@@ -380,15 +380,20 @@ void accum(float* a, float* b, int size) {
 
 // ------------------------------------------------------- KV block pool
 // Host bookkeeping exactly as reference memory.c:8-82; the two pools are HBM.
-static void init_free_stack(KVCacheManager* mgr, int block_size, int num_blocks) {
+static bool try_free_stack(KVCacheManager* mgr, int block_size, int num_blocks) {   // false: no memory
     mgr->block_size = block_size;
     mgr->num_blocks = num_blocks;
     mgr->free_blocks_count = num_blocks;
     mgr->free_block_indices = (int*)malloc((size_t)num_blocks * sizeof(int));
+    if (!mgr->free_block_indices) return false;
     for (int slot = 0; slot < num_blocks; slot++) mgr->free_block_indices[slot] = num_blocks - 1 - slot;
     WITH_POOLS;   // (what is known of a manager whose stack lay here)
     attached().erase(mgr->free_block_indices);
     forget_shared_blocks(mgr->free_block_indices);
+    return true;
+}
+static void init_free_stack(KVCacheManager* mgr, int block_size, int num_blocks) {
+    if (!try_free_stack(mgr, block_size, num_blocks) && num_blocks > 0) NVLLM_FATAL("cannot allocate the free stack of %d blocks", num_blocks);
 }
 
 void init_kv_cache_manager(KVCacheManager* mgr, int block_size, int num_blocks, int n_layers,
@@ -430,7 +435,7 @@ int nvllm_attach_kv_pool(KVCacheManager* mgr, int block_size, int num_blocks, in
     if ((long)num_blocks * block_size > 0x7fffffff) return NVLLM_BAD_SIZE;   // (rows of a pool are ints)
     if (((size_t)pool_k | (size_t)pool_v) % 16) return NVLLM_BAD_ARGUMENT;
     KVCacheManager m = *mgr;
-    init_free_stack(&m, block_size, num_blocks);
+    if (!try_free_stack(&m, block_size, num_blocks)) return NVLLM_NO_MEMORY;
     m.pool_k = (float*)pool_k;
     m.pool_v = (float*)pool_v;
     int refusal = 0;

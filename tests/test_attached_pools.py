@@ -77,3 +77,15 @@ release(a)
 assert users(b, 3) == [2, 2, 0] and fork(b, u, 16)[0] == 0 and users(b, 3) == [3, 2, 0]
 release(b)
 """)
+
+
+def test_a_free_stack_without_memory():
+    """The host's own memory: a pool whose free stack the system does not give."""
+    run("""
+import resource
+resource.setrlimit(resource.RLIMIT_AS, (8 << 30, 8 << 30))
+m = capi.KVCacheManager()
+assert lib.nvllm_attach_kv_pool(C.byref(m), 1, 0x7fffffff, 1, 1, 1, 4, 0x100000, 0x100000000) == -5
+assert not m.free_block_indices and not m.pool_k
+release(attach(blocks=1000))
+""")
