@@ -345,8 +345,11 @@ __device__ __forceinline__ Portion portion_of(const DeltaChunks& c, int s) {
     Portion p = {c.a.here[at], c.first_here[at]};
     ASKED_FOR_AT_ONCE(c.a);
     asm volatile("" ::"s"(p.span.x), "s"(p.span.y), "s"(p.span.z), "s"(p.span.w), "s"(p.first), "s"(c.mem), "s"(c.first), "s"(c.from), "s"(c.most), "s"(c.segs), "s"(c.per_seg), "s"(c.out_four),
-                 "s"(c.a.out), "s"(c.a.v_cols), "s"(c.a.dim_kept));
-    if (c.a.spans) p = {c.a.spans[s], c.first[s]};
+                 "s"(c.a.out), "s"(c.a.v_cols), "s"(c.a.dim_kept), "s"(c.a.n_spans));
+    if (c.a.spans) {   // (s may be a segment's number: those go further than portions, whose own is looked up then)
+        const int own = min(s, c.a.n_spans - 1);
+        p = {c.a.spans[own], c.first[own]};
+    }
     return {scalars(p.span), __builtin_amdgcn_readfirstlane(p.first)};
 }
 struct ChunkAt {
