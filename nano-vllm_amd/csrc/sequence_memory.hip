@@ -35,6 +35,7 @@ struct CopySet {
 struct CopyArgs {
     CopySet sets[COPY_SETS];
     int n_programs;
+    unsigned piece;               // of every slot, the launch's first
     const int* programs;          // null: the ints are right here
     int here[COPY_INLINE];        // [n_programs + 1] first moves, then moves (from, to)
 };
@@ -49,7 +50,7 @@ __device__ __forceinline__ void store_past_caches(U* p, const U& v) {
 template <typename U, int N, bool HERE>
 __global__ __launch_bounds__(256) void k_copy_slots(CopyArgs a) {
     const int array = blockIdx.y, program = blockIdx.x % a.n_programs;
-    const unsigned first = (blockIdx.x / a.n_programs) * (256 * N) + threadIdx.x;
+    const unsigned first = (a.piece + blockIdx.x / a.n_programs) * (256 * N) + threadIdx.x;
     CopySet set = a.sets[0];
 #pragma unroll
     for (int i = 1; i < COPY_SETS; i++)   // (sets that are not there begin behind the last array)
@@ -219,13 +220,20 @@ static int plan_moves(const int* from, const int* to, int n, int n_slots, CopyPl
     return 0;
 }
 
+constexpr long GRID_MOST = 0xffffffffL / 256;   // workgroups: a grid has fewer than 2^32 threads
+
 template <typename U>
-static void launch_copy(const CopyArgs& a, unsigned most_units, int arrays) {
+static void launch_copy(CopyArgs& a, unsigned most_units, int arrays, double bytes) {
     constexpr int N = 2;
-    const long pieces = (most_units + 256 * N - 1) / (256 * N);
-    const dim3 grid((unsigned)(pieces * a.n_programs), arrays);
-    if (a.programs) NVLLM_LAUNCH((k_copy_slots<U, N, false>), grid, dim3(256), 0, a);
-    else NVLLM_LAUNCH((k_copy_slots<U, N, true>), grid, dim3(256), 0, a);
+    const long pieces = ((long)most_units + 256 * N - 1) / (256 * N), at_once = std::max(1L, std::min(pieces, GRID_MOST / a.n_programs));
+    for (long p = 0; p < pieces; p += at_once) {
+        a.piece = (unsigned)p;
+        const long n = std::min(at_once, pieces - p);
+        const dim3 grid((unsigned)(n * a.n_programs), arrays);
+        ProfScope ps(PC_SLOT_COPY, bytes * n / pieces, 0);
+        if (a.programs) NVLLM_LAUNCH((k_copy_slots<U, N, false>), grid, dim3(256), 0, a);
+        else NVLLM_LAUNCH((k_copy_slots<U, N, true>), grid, dim3(256), 0, a);
+    }
 }
 
 int copy_slots(const std::vector<SlotArrays>& arrays, int n_slots, const int* from, const int* to, int n) {
@@ -240,7 +248,7 @@ int copy_slots(const std::vector<SlotArrays>& arrays, int n_slots, const int* fr
     }
     const size_t unit = bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 1;
     for (const SlotArrays& s : arrays)
-        if (s.slot_bytes / unit > 0x7fffffff || (double)(s.slot_bytes / unit / 512 + 1) * (double)plan.programs() > 2e9) return NVLLM_BAD_SIZE;
+        if (s.slot_bytes / unit > 0x7fffffff) return NVLLM_BAD_SIZE;
     if (ints + 4 > staging_ints()) return NVLLM_BAD_SIZE;
     ensure_init();
     if (stream_is_captured()) return NVLLM_CAPTURED;
@@ -270,10 +278,9 @@ int copy_slots(const std::vector<SlotArrays>& arrays, int n_slots, const int* fr
         }
         for (int j = sets; j < COPY_SETS; j++) a.sets[j] = CopySet{nullptr, 0, 0, 0x7fffffff};
         if (total == 0) continue;
-        ProfScope ps(PC_SLOT_COPY, part, 0);
-        if (unit == 16) launch_copy<uint4>(a, most, total);
-        else if (unit == 4) launch_copy<unsigned>(a, most, total);
-        else launch_copy<unsigned char>(a, most, total);
+        if (unit == 16) launch_copy<uint4>(a, most, total, part);
+        else if (unit == 4) launch_copy<unsigned>(a, most, total, part);
+        else launch_copy<unsigned char>(a, most, total, part);
     }
     return 0;
 }
