@@ -1140,13 +1140,14 @@ __global__ __launch_bounds__(64 * join_waves<DC>()) void k_delta_join(DeltaChunk
 // Rows of queries and keys whose dims or addresses the chunk kernels' loads do not fit: dims padded to a multiple of 8 with zeros.
 // (The same for values.)
 template <typename E>
-__global__ __launch_bounds__(256) void k_delta_rows(E* __restrict__ dst, const E* __restrict__ src, int Q, int dim, int dim_ld, long ld) {
-    const long row = blockIdx.x;
-    for (int i = threadIdx.x; i < Q * dim_ld; i += 256) {
-        const int hq = i / dim_ld, d = i - hq * dim_ld;
-        dst[row * Q * dim_ld + i] = d < dim ? src[row * ld + hq * dim + d] : (E)0;
-    }
+__global__ __launch_bounds__(256) void k_delta_rows(E* __restrict__ dst, const E* __restrict__ src, int T, int Q, int dim, int dim_ld, long ld) {
+    for (long row = blockIdx.x; row < T; row += gridDim.x)
+        for (int i = threadIdx.x; i < Q * dim_ld; i += 256) {
+            const int hq = i / dim_ld, d = i - hq * dim_ld;
+            dst[row * Q * dim_ld + i] = d < dim ? src[row * ld + hq * dim + d] : (E)0;
+        }
 }
+constexpr int ROWS_GRID = 1 << 20;   // its workgroups at most (a grid has fewer than 2^32 threads)
 
 template <typename F>
 static void more_lds(F* kernel, int bytes) {
@@ -1338,8 +1339,9 @@ static int gated_delta(Delta& a, const int* seq_ids, const int* pos, int T, int 
         c.a = a;
         c.out_four = a.vdim % 4 == 0 && (size_t)a.out % (4 * elem) == 0;
         auto pack = [&](const void*& src, long& ld, int heads, int dim, int wide) {
-            if (b16) NVLLM_LAUNCH((k_delta_rows<unsigned short>), dim3(T), dim3(256), 0, (unsigned short*)mem, (const unsigned short*)src, heads, dim, wide, ld);
-            else NVLLM_LAUNCH((k_delta_rows<float>), dim3(T), dim3(256), 0, (float*)mem, (const float*)src, heads, dim, wide, ld);
+            const dim3 grid(std::min(T, ROWS_GRID));
+            if (b16) NVLLM_LAUNCH((k_delta_rows<unsigned short>), grid, dim3(256), 0, (unsigned short*)mem, (const unsigned short*)src, T, heads, dim, wide, ld);
+            else NVLLM_LAUNCH((k_delta_rows<float>), grid, dim3(256), 0, (float*)mem, (const float*)src, T, heads, dim, wide, ld);
             src = mem;
             ld = (long)heads * wide;
         };

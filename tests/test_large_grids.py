@@ -22,3 +22,13 @@ unit = 16 if slot %% 16 == 0 else 4 if slot %% 4 == 0 else 1
 work = [g for g, b in launches() if g[1] == 2]
 assert sum(g[0] for g in work) == n * -(-slot // unit // 512)   # every piece of every move once
 """ % (slot, n))
+
+
+@pytest.mark.parametrize("tokens", [1 << 24, (1 << 24) + 5], ids=str)
+def test_packed_rows(tmp_path, tokens):
+    """A portion of 16 million tokens whose rows are packed, a workgroup a row."""
+    hip_standin.run(tmp_path, CHECK + """
+n = %d
+assert delta(np.zeros(n), np.arange(n), 1, 1, 5, 3) == 0
+fits()
+""" % tokens)
