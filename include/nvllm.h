@@ -201,9 +201,9 @@ int nvllm_compact_blocks(KVCacheManager* mgr, BlockTable** tables, int n);
 
 /* A pool in memory of the caller's (16-byte aligned, HBM): [n_layers][num_blocks][block_size][n_kv_heads][head_dim] elements each for
  * keys and values, fp32 rows (elem_bytes 4) or fp16 pages (2; block_size 16, head_dim a multiple of 16, whose values have to be
- * finite from the start).  Used like one of init_kv_cache_manager(); free_kv_cache_manager() leaves the memory alone.  n_kv_heads: the
- * heads that this process stores.  Memory that is attached again is the later manager's: the earlier one's tables can be freed and
- * itself released, copies, forks and compaction refuse it (NVLLM_BAD_SIZE). */
+ * finite from the start).  Used like one of init_kv_cache_manager(); free_kv_cache_manager() leaves the memory alone and returns when
+ * nothing that was enqueued uses it any more.  n_kv_heads: the heads that this process stores.  Memory that is attached again is the
+ * later manager's: the earlier one's tables can be freed and itself released, copies, forks and compaction refuse it (NVLLM_BAD_SIZE). */
 int nvllm_attach_kv_pool(KVCacheManager* mgr, int block_size, int num_blocks, int n_layers, int n_kv_heads, int head_dim, int elem_bytes, void* pool_k, void* pool_v);
 
 /* -------------------------------------------------- one launch per decode step */

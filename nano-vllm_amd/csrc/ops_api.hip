@@ -488,6 +488,9 @@ void free_kv_cache_manager(KVCacheManager* mgr) {
     if (owned) {
         device_free(mgr->pool_k);
         device_free(mgr->pool_v);
+    } else if (rt().inited) {   // (the caller may free it next; nothing of a captured stream runs yet)
+        ensure_init();
+        if (!stream_is_captured()) sync_streams();
     }
     mgr->pool_k = mgr->pool_v = nullptr;
 }

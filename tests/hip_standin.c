@@ -11,7 +11,7 @@ static size_t n_launches, room;
 static size_t memory = (size_t)288 << 30, taken, largest, frees;
 static uintptr_t next_at = 0x100000000000;
 static struct { uintptr_t at; size_t bytes; } blocks[4096];
-static int n_blocks, sticky, capturing;
+static int n_blocks, sticky, capturing, waits;
 
 /* ---- what a test reads and sets */
 void standin_memory(size_t bytes) { memory = bytes; }
@@ -19,6 +19,7 @@ void standin_capture(int on) { capturing = on; }
 size_t standin_taken(void) { return taken; }
 size_t standin_largest(void) { return largest; }
 size_t standin_frees(void) { return frees; }
+int standin_waits(void) { return waits; }   /* for a stream */
 size_t standin_launches(void) { return n_launches; }
 void standin_launch(size_t i, unsigned long* six) { memcpy(six, &launches[i], sizeof(launch_t)); }
 void standin_forget(void) { n_launches = largest = 0; }
@@ -75,7 +76,7 @@ hipError_t hipGetDevicePropertiesR0600(hipDeviceProp_tR0600* p, int d) {
 hipError_t hipGetSymbolAddress(void** p, const void* symbol) { return *p = (void*)0x7000000, hipSuccess; }
 hipError_t hipFuncSetAttribute(const void* f, hipFuncAttribute a, int v) { return hipSuccess; }
 hipError_t hipStreamCreateWithFlags(hipStream_t* s, unsigned flags) { return *s = (hipStream_t)0x10, hipSuccess; }
-hipError_t hipStreamSynchronize(hipStream_t s) { return hipSuccess; }
+hipError_t hipStreamSynchronize(hipStream_t s) { return waits++, capturing ? hipErrorStreamCaptureUnsupported : hipSuccess; }
 hipError_t hipStreamIsCapturing(hipStream_t s, hipStreamCaptureStatus* st) { return *st = capturing ? hipStreamCaptureStatusActive : hipStreamCaptureStatusNone, hipSuccess; }
 hipError_t hipEventCreate(hipEvent_t* e) { return *e = (hipEvent_t)0x20, hipSuccess; }
 hipError_t hipEventCreateWithFlags(hipEvent_t* e, unsigned flags) { return *e = (hipEvent_t)0x20, hipSuccess; }
