@@ -1,5 +1,5 @@
 // sequence_memory.h -- what sequences remember, moved as a whole: blocks of a paged cache and states of slots, copied in every
-// layer by one launch.
+// layer together: a launch takes six sets of arrays (a pool of keys and values is two), and as many pieces as a grid has room for.
 #pragma once
 
 #include <vector>

@@ -339,7 +339,8 @@ static std::vector<char> free_blocks(const KVCacheManager* mgr) {
     return is_free;
 }
 // A table's release: how many blocks go back to the pool; a refusal for a table that names a block twice, or one that is free.  A shared block is
-// in use; the free stack, which the caller may write too, is read for the others: 0.2 us for 512 free blocks, 3 for 8,192.
+// in use; the free stack, which the caller may write too, is read for the others (a release of 33 blocks: 0.4 us beside 512 free ones, 2.0 beside
+// 8,192).
 static int blocks_to_free(const KVCacheManager* mgr, const BlockTable* table, const std::vector<int>* users) {
     const unsigned n = (unsigned)mgr->num_blocks;
     static thread_local std::vector<unsigned char> marks;   // all zeros between calls
