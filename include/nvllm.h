@@ -141,7 +141,7 @@ void nvllm_expert_ff(float* out, int* choice, float* score, const float* in, con
  * q and k divided by sqrt(sum of their squares + norm_eps) first when norm_eps > 0.  state: fp32 [n_slots][heads][dim][vdim], a
  * sequence's slot is its id in seq_ids, empty at position 0; slots that the batch does not name stay as they are.  q, k: rows of
  * [qk_heads][dim], v: rows of [heads][vdim], the first of token t at element t * q_ld, t * k_ld, t * v_ld; out [num_tokens][heads][vdim];
- * elem_bytes 4: fp32, 2: bf16 (out is rounded once).  g (logarithm of the decay, at most 0; -infinity empties the state) and beta: fp32
+ * elem_bytes 4: fp32, 2: bf16 (out is rounded once).  g (logarithm of the decay, at most 0; -infinity empties a state of finite values) and beta: fp32
  * [num_tokens][heads].  A sequence's tokens lie side by side at consecutive positions.  States and all sums in fp32.
  * dim at most 256, heads and vdim at most 65,535, heads * vdim and the strides at most 2^23.  out and state overlap nothing else.
  * Portions go in chunks of 64 tokens from some length on (10 to 75 tokens, by the batch's size and type), whose products run over whole chunks: a
